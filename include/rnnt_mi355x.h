@@ -240,6 +240,59 @@ int rnnt_mi355x_joint_log_softmax(const float* f, int f_rows, const float* g, in
                                   const int32_t* g_index, int n_rows, int V, float* out, int32_t* bad_index_flag,
                                   void* hip_stream);
 
+/* ---- operators around the joint network: dropout, beam step ----------------------
+ * They take float32, bfloat16 and float16 tensors (`dtype`); every sum, softmax statistic
+ * and score is held in 32 bits or more. */
+#define RNNT_MI355X_FP32 0
+#define RNNT_MI355X_BF16 1
+#define RNNT_MI355X_FP16 2
+
+/* y = x * m / keep for the Dropout layers of get_fc (reference
+ * rnnt/keras_model.py:102-103), keep = 1 - drop16/65536.  x: [rows, cols], rows
+ * x_stride >= cols elements apart; y: dense, may be x itself when x_stride ==
+ * cols.  The mask is drawn, never stored: element (r, c) uses bits
+ * 16*(c%2) .. +15 of word (c%8)/2 of Philox4x32-10 at counter (c/8, r, offset low,
+ * offset high), key (seed low, seed high), and is kept when they are >= drop16.
+ * The backward pass is the same call on the upstream gradient.  offset_dev
+ * (nullable, device) replaces `offset`: a captured graph draws a new mask on every
+ * replay when the caller advances it. */
+int rnnt_mi355x_dropout(const void* x, long long x_stride, void* y, long long rows, int cols, int dtype, int drop16,
+                        uint64_t seed, uint64_t offset, const uint64_t* offset_dev, void* hip_stream);
+
+/* One step of a beam search (what reference rnnt/rnnt_decoder.py:95-233 does with the
+ * log-probabilities of its inner step).  logits: [B, K, V] (last dimension
+ * contiguous, strides in elements), enc: [B, V] or NULL, added to the logits of all
+ * beams of an utterance (sum rounded to float32); scores: [B, K]; allowed: bytes
+ * [B, V] or NULL, zero forbids a symbol (its logit is not looked at and has no part in
+ * the softmax; allowed_batch_stride 0: one mask for all utterances); finished: bytes
+ * [B, K] or NULL: such a beam offers itself alone, with its score, at symbol `end`.
+ *   total = scores + x - log sum exp x          (ordered in float64)
+ * and the `width` largest totals of an utterance, ties to the lowest k*V + v, go to
+ * out_scores / out_parent / out_token [B, width]; places without a candidate hold
+ * -inf, -1, -1.  A beam whose score is NaN or beyond +-2^30 is empty; so is one whose
+ * allowed logits hold a NaN or +inf, or nothing above -inf.  K, width <= 64,
+ * K*V < 2^31.  `workspace`: rnnt_mi355x_beam_select_workspace_bytes (0: may be NULL). */
+int rnnt_mi355x_beam_select_workspace_bytes(int B, int K, int V, int width, size_t* out_bytes);
+int rnnt_mi355x_beam_select(const void* logits, long long logits_batch_stride, long long logits_beam_stride, int dtype,
+                            const void* enc, long long enc_batch_stride, const float* scores, const uint8_t* allowed,
+                            long long allowed_batch_stride, const uint8_t* finished, int end, int B, int K, int V,
+                            int width, float* out_scores, int32_t* out_parent, int32_t* out_token, void* workspace,
+                            void* hip_stream);
+
+/* dst[o, b, w, :] = src[o, b, parent[b, w], :], zeros where parent is outside [0, K):
+ * the hypotheses' network states in the order beam_select gave them, up to
+ * RNNT_MI355X_REORDER_MAX tensors in one launch.  src: rows of row_bytes bytes at
+ * the byte strides given; dst: dense [outer, B, width, row_bytes], not
+ * overlapping any src. */
+#define RNNT_MI355X_REORDER_MAX 16
+typedef struct {
+  const void* src;
+  void* dst;
+  long long outer, outer_stride, batch_stride, beam_stride, row_bytes; /* strides in bytes */
+} rnnt_mi355x_reorder_tensor;
+int rnnt_mi355x_beam_reorder(const rnnt_mi355x_reorder_tensor* tensors, int n_tensors, const int32_t* parent, int B,
+                             int K, int width, void* hip_stream);
+
 /* out2[0] = sum_b costs[b], out2[1] = sum of squared gradient elements of the
  * last backward on this workspace (both float64, device memory).  These are
  * the two scalars a data-parallel caller all-reduces: the batch loss of

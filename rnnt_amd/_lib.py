@@ -41,6 +41,14 @@ _lib = None
 
 _vp, _i, _sz, _ll, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong, ctypes.c_float
 _META = [_i] * 5  # B, maxT, maxU1, V, blank
+_u64 = ctypes.c_uint64
+REORDER_MAX = 16  # RNNT_MI355X_REORDER_MAX
+
+
+class ReorderTensor(ctypes.Structure):
+    """rnnt_mi355x_reorder_tensor"""
+    _fields_ = [("src", _vp), ("dst", _vp)] + [(n, _ll) for n in ("outer", "outer_stride", "batch_stride", "beam_stride", "row_bytes")]
+
 
 _SIGNATURES = {
     "rnnt_mi355x_workspace_bytes": (ctypes.c_int, [_i, _i, _i, ctypes.POINTER(_sz)]),
@@ -67,6 +75,10 @@ _SIGNATURES = {
     "rnnt_mi355x_dense_forward": (ctypes.c_int, [_vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp]),
     "rnnt_mi355x_dense_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "rnnt_mi355x_joint_log_softmax": (ctypes.c_int, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "rnnt_mi355x_dropout": (ctypes.c_int, [_vp, _ll, _vp, _ll, _i, _i, _i, _u64, _u64, _vp, _vp]),
+    "rnnt_mi355x_beam_select_workspace_bytes": (ctypes.c_int, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "rnnt_mi355x_beam_select": (ctypes.c_int, [_vp, _ll, _ll, _i, _vp, _ll, _vp, _vp, _ll, _vp] + [_i] * 5 + [_vp] * 5),
+    "rnnt_mi355x_beam_reorder": (ctypes.c_int, [ctypes.POINTER(ReorderTensor), _i, _vp, _i, _i, _i, _vp]),
     "rnnt_mi355x_reduce_scalars": (ctypes.c_int, [_vp, _i, _vp, _vp, _vp]),
     "rnnt_mi355x_read_status": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int32), _vp]),
     "rnnt_mi355x_status_string": (ctypes.c_char_p, [_i]),

@@ -13,15 +13,21 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 SOURCES = [os.path.join(CSRC, "rnnt_mi355x.hip"), os.path.join(CSRC, "fc_joint.hip"),
            os.path.join(CSRC, "skinny_dense.hip"), os.path.join(CSRC, "decode_step.hip")]
+# operators around the joint network
+OPERATOR_SOURCES = [os.path.join(CSRC, "dropout.hip"), os.path.join(CSRC, "beam.hip")]
+OPERATOR_PIECES = [os.path.join(CSRC, "op_util.h")]
 # rnnt_mi355x.hip is one translation unit whose kernels live in these included pieces
 PIECES = [os.path.join(CSRC, n) for n in ("workspace.h", "device_util.h", "lse_rows.h", "sweep.h", "grad_rows.h", "grad_span.h", "grad_split.h", "cell_coef.h", "grad_flat.h", "lse_span.h",
                                           "small_vocab.h", "joint.h", "aux_kernels.h")]
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "rnnt_mi355x.h")
 LIB = os.path.join(CSRC, "librnnt_mi355x.so")
+# hipcc's packed float32 instructions have given wrong results on this hardware now and then: no source is built with them
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Xclang", "-target-feature", "-Xclang",
+         "-packed-fp32-ops"]
 
 
 def sources_digest() -> str:
-    """Sixteen hex digits that change whenever a kernel source changes: measurements taken from a build (the HBM
+    """Sixteen hex digits that change whenever a source of the loss and its joints changes: measurements taken from a build (the HBM
     counter bytes of profiles/traffic.json) are stamped with it and not quoted for another one."""
     import hashlib
     h = hashlib.sha256()
@@ -42,15 +48,15 @@ def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(p) > t for p in (*SOURCES, *PIECES, HEADER))
+    return any(os.path.getmtime(p) > t for p in (*SOURCES, *PIECES, *OPERATOR_SOURCES, *OPERATOR_PIECES, HEADER))
 
 
 def newer_sources():
     """Sources that are newer than the built library."""
     if not os.path.exists(LIB):
-        return [*SOURCES]
+        return [*SOURCES, *OPERATOR_SOURCES]
     t = os.path.getmtime(LIB)
-    return [p for p in (*SOURCES, *PIECES, HEADER) if os.path.getmtime(p) > t]
+    return [p for p in (*SOURCES, *PIECES, *OPERATOR_SOURCES, *OPERATOR_PIECES, HEADER) if os.path.getmtime(p) > t]
 
 
 def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB) -> str:
@@ -70,11 +76,12 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB
         try:
             if not force and out == LIB and not needs_build():  # another process built it while this one waited
                 return LIB
-            flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", *[f"-D{d}" for d in defines]]
+            flags = [*FLAGS, *[f"-D{d}" for d in defines]]
             with tempfile.TemporaryDirectory(prefix=".build-", dir=os.path.dirname(out)) as tmp:
                 # one object per source, compiled side by side, then one link
-                objs = [os.path.join(tmp, os.path.splitext(os.path.basename(src))[0] + ".o") for src in SOURCES]
-                cmds = [[hipcc, *flags, "-c", src, "-o", obj] for src, obj in zip(SOURCES, objs)]
+                sources = [*SOURCES, *OPERATOR_SOURCES]
+                objs = [os.path.join(tmp, os.path.splitext(os.path.basename(src))[0] + ".o") for src in sources]
+                cmds = [[hipcc, *flags, "-c", src, "-o", obj] for src, obj in zip(sources, objs)]
                 if verbose:
                     for cmd in cmds:
                         print(" ".join(cmd))

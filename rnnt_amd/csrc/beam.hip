@@ -1,0 +1,593 @@
+// One step of a beam search for MI355X (gfx950): selection over beams x vocabulary, and the hypotheses' states in their
+// new order.  Where the reference's decoder scores one hypothesis at a time in numpy (reference
+// rnnt/rnnt_decoder.py:156-158, 200-202) and sorts them on the host, here
+//     x[b,k,v]     = logits[b,k,v] (+ enc[b,v], rounded to float32)
+//     total[b,k,v] = scores[b,k] + x[b,k,v] - log sum_v' exp x[b,k,v'],      v' over the allowed symbols
+// and the `width` largest totals of an utterance, ties to the lowest k * V + v.
+//
+// A wavefront takes a piece of a row into registers, at most 32 values a lane.  Inside a row the order of the totals is
+// the order of x, so a piece needs only its own `width` largest x (exact float32 comparisons) and its share of the
+// softmax sum; the totals themselves are formed in float64, because candidates of different beams lie arbitrarily close
+// and a float32 sum would order them by its rounding.
+//   - the lanes' maxima are sorted across the wavefront; the width-th of them is a lower bound T of the width-th largest
+//     value, and the few values >= T are compacted and sorted (64 at a time, a bitonic network over the lanes);
+//   - sorted lists are joined by the first step of a bitonic merge: of two sorted lists a, b the values
+//     max(a[i], b[P-1-i]) are the P largest, and log2 P exchanges sort them.
+// Rows of up to 2048 symbols take one launch, a block per utterance; longer ones a launch over pieces of 2048 and one that
+// joins the pieces' lists.
+#include "op_util.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = 1.925963033500924e-8f;  // log2 e - (float)log2 e
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kScoreLimit = 1073741824.f;  // 2^30: a score beyond it marks an empty beam (or is no score at all)
+constexpr int kMaxBeams = 64, kMaxWidth = 64;
+constexpr int kPiece = 2048;  // symbols of a row that one wavefront takes
+
+// ---- exchanges between lanes --------------------------------------------------------------------------------------------
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (M == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);        // quad_perm 1,0,3,2
+  else if constexpr (M == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // quad_perm 2,3,0,1
+  else if constexpr (M == 3) return __builtin_amdgcn_update_dpp(0, v, 0x1B, 0xf, 0xf, true);   // quad_perm 3,2,1,0
+  else if constexpr (M == 7) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (M == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);  // row_ror:8
+  else if constexpr (M == 15) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true); // row_mirror
+  else if constexpr (M == 4) return lane_xor<7>(lane_xor<3>(v));
+  else return __shfl_xor(v, M, 64);
+}
+
+// Candidates: larger is better, all of them different; zero stands for none.
+struct RowKey {  // value of a row, then the lower symbol
+  uint32_t hi, lo;
+  __device__ __forceinline__ bool operator>(const RowKey& o) const {
+    return (((uint64_t)hi << 32) | lo) > (((uint64_t)o.hi << 32) | o.lo);
+  }
+};
+struct TotalKey {  // total in float64, then the lower place in beams x vocabulary
+  uint64_t hi;
+  uint32_t lo;
+  __device__ __forceinline__ bool operator>(const TotalKey& o) const { return hi > o.hi || (hi == o.hi && lo > o.lo); }
+};
+template <int M>
+__device__ __forceinline__ RowKey lane_xor(const RowKey& k) {
+  return {lane_xor<M>(k.hi), lane_xor<M>(k.lo)};
+}
+template <int M>
+__device__ __forceinline__ TotalKey lane_xor(const TotalKey& k) {
+  return {((uint64_t)lane_xor<M>((uint32_t)(k.hi >> 32)) << 32) | lane_xor<M>((uint32_t)k.hi), lane_xor<M>(k.lo)};
+}
+// order-preserving integers of floating values (no NaN comes here; every finite or infinite value gives more than zero)
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return b ^ ((int32_t)b >> 31 | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double unordered(uint64_t k) {
+  return __builtin_bit_cast(double, k >> 63 ? k ^ 0x8000000000000000ull : ~k);
+}
+
+// The lane whose index has bit log2(D) clear keeps the larger key.
+template <int M, int D, class K>
+__device__ __forceinline__ void exchange(K& k, int lane) {
+  const K o = lane_xor<M>(k);
+  if ((o > k) == !(lane & D)) k = o;
+}
+// In each list of P lanes a bitonic sequence becomes a descending one.
+template <int P, class K>
+__device__ __forceinline__ void clean(K& k, int lane) {
+  if constexpr (P >= 64) exchange<32, 32>(k, lane);
+  if constexpr (P >= 32) exchange<16, 16>(k, lane);
+  if constexpr (P >= 16) exchange<8, 8>(k, lane);
+  if constexpr (P >= 8) exchange<4, 4>(k, lane);
+  if constexpr (P >= 4) exchange<2, 2>(k, lane);
+  if constexpr (P >= 2) exchange<1, 1>(k, lane);
+}
+// 64 keys in descending order over the lanes: at every stage two sorted runs are joined by their mirrored exchange.
+template <class K>
+__device__ __forceinline__ void sort64(K& k, int lane) {
+  exchange<1, 1>(k, lane);
+  exchange<3, 2>(k, lane);  clean<2>(k, lane);
+  exchange<7, 4>(k, lane);  clean<4>(k, lane);
+  exchange<15, 8>(k, lane); clean<8>(k, lane);
+  exchange<31, 16>(k, lane); clean<16>(k, lane);
+  exchange<63, 32>(k, lane); clean<32>(k, lane);
+}
+// acc and a list that comes in reverse order, P lanes a list: acc becomes the P largest of both.
+template <int P, class K>
+__device__ __forceinline__ void join(K& acc, const K& reversed, int lane) {
+  if (reversed > acc) acc = reversed;
+  clean<P>(acc, lane);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// What a wavefront's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+struct BeamArgs {
+  const void* logits;
+  const void* enc;         // nullable
+  const float* scores;     // [B, K]
+  const uint8_t* allowed;  // nullable
+  const uint8_t* finished; // nullable, [B, K]
+  long long logits_b, logits_k, enc_b, allowed_b;  // strides in elements
+  int B, K, V, width, end, pieces;
+  float* out_scores;
+  int32_t *out_parent, *out_token;
+};
+
+// The piece [v0, v0 + 64 * E) of a row in registers: element j*64*W + lane*W + i of it, W = 4 or 8 consecutive ones.
+// Symbols past V and forbidden ones are -inf whatever the memory holds.
+template <class T, int E>
+__device__ __forceinline__ void load_piece(const BeamArgs& a, int b, int k, int v0, int lane, float (&x)[E]) {
+  const typename T::elem* row = static_cast<const typename T::elem*>(a.logits) + b * a.logits_b + k * a.logits_k;
+  const typename T::elem* enc = a.enc ? static_cast<const typename T::elem*>(a.enc) + b * a.enc_b : nullptr;
+  const uint8_t* allowed = a.allowed ? a.allowed + b * a.allowed_b : nullptr;
+  constexpr int G = E / 8;
+  Raw8<T> r[G], e[G];
+  u2 m[G];
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int v = v0 + j * 512 + lane * 8;
+    if (v + 8 <= a.V) {
+      r[j] = load8_raw<T>(row + v);
+      if (enc) e[j] = load8_raw<T>(enc + v);
+      if (allowed) __builtin_memcpy(&m[j], allowed + v, 8);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int v = v0 + j * 512 + lane * 8;
+    float y[8];
+    if (v + 8 <= a.V) {
+      unpack8<T>(r[j], y);
+      if (enc) {
+        float z[8];
+        unpack8<T>(e[j], z);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] += z[i];
+      }
+      if (allowed) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (m[j][i >> 2] >> (8 * (i & 3))) & 0xffu ? y[i] : -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = -INFINITY;
+        if (v + i < a.V) {
+          const float t = to_float<T>(row[v + i]) + (enc ? to_float<T>(enc[v + i]) : 0.f);
+          if (!allowed || allowed[v + i]) y[i] = t;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[8 * j + i] = y[i] + 0.f;  // -0 becomes +0: the two tie
+  }
+}
+
+// Softmax share and the 64 best candidates of a piece: *m the largest value, *s = sum exp(x - m) (NaN when a value is NaN
+// or +inf), and in lane i the i-th candidate, of which the first `width` are right.  buf: 128 keys of LDS of this wavefront.
+template <int E>
+__device__ __forceinline__ RowKey best_of_piece(const float (&x)[E], int v0, int width, int lane, RowKey* buf, float* m, double* s) {
+  float top = -INFINITY;
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (x[e] > top) {
+      top = x[e];
+      at = (e >> 3) * 512 + lane * 8 + (e & 7);
+    }
+  const float mx = wave_max(top);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  double sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    // exp(x - m) to about one unit in the last place: the difference and its product with log2 e with their rounding
+    // errors (the sum decides between candidates of different beams)
+    const float d = x[e] - base, bb = d - x[e], err = (x[e] - (d - bb)) - (base + bb);
+    const float t = d * kLog2e;
+    const float low = fmaf(err, kLog2e, fmaf(d, kLog2eLow, fmaf(d, kLog2e, -t)));
+    const float p = __builtin_amdgcn_exp2f(t);
+    // below 2^-160 the term is zero, also where x = -inf or the difference overflows and the corrections are NaN; a NaN
+    // among the values stays one
+    const float term = t < -160.f ? 0.f : fmaf(p * kLn2, low, p);
+    sum += (double)term;
+  }
+  *m = mx;
+  *s = wave_sum(sum);
+
+  RowKey lanes = {0u, 0u};
+  if (top > -INFINITY) lanes = {ordered(top), ~(uint32_t)(v0 + at)};
+  sort64(lanes, lane);
+  const RowKey bound = {(uint32_t)__shfl((int)lanes.hi, width - 1, 64), (uint32_t)__shfl((int)lanes.lo, width - 1, 64)};
+  const float floor_x = bound.hi ? unordered(bound.hi) : -INFINITY;
+  RowKey acc = {0u, 0u};
+  int fill = 0;
+  bool first = true;
+  auto take = [&](int n) {  // the first n <= 64 keys of the buffer join acc
+    wave_sync();
+    RowKey k = {0u, 0u};
+    if (lane < n) k = buf[lane];
+    sort64(k, lane);
+    if (first) acc = k;
+    else join<64>(acc, lane_xor<63>(k), lane);
+    first = false;
+  };
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const RowKey k = {ordered(x[e]), ~(uint32_t)(v0 + (e >> 3) * 512 + lane * 8 + (e & 7))};
+    const bool in = x[e] >= floor_x && x[e] > -INFINITY && !(bound > k);
+    const uint64_t who = __ballot(in);
+    if (who) {  // uniform
+      if (in) buf[fill + __popcll(who & ((1ull << lane) - 1))] = k;
+      fill += __popcll(who);
+      if (fill >= 64) {
+        take(64);
+        RowKey rest = {0u, 0u};
+        if (lane < fill - 64) rest = buf[64 + lane];
+        wave_sync();
+        if (lane < fill - 64) buf[lane] = rest;
+        fill -= 64;
+      }
+    }
+  }
+  if (fill > 0) take(fill);
+  return acc;
+}
+
+__device__ __forceinline__ bool live_score(float s) { return fabsf(s) <= kScoreLimit; }
+
+// A row's softmax: the largest value and log sum exp(x - m).
+struct RowSum {
+  double m, log_s;
+};
+
+// The candidate c of beam k, or the one of a finished beam, in the order of the utterance.
+__device__ __forceinline__ TotalKey total_key(const BeamArgs& a, int k, bool done, float score, const RowSum& row, const RowKey& c) {
+  TotalKey t = {0ull, 0u};
+  if (done) {
+    t.hi = ordered((double)score + 0.0);
+    t.lo = ~(uint32_t)(k * a.V + a.end);
+  } else if (c.hi) {
+    t.hi = ordered((double)score + (((double)unordered(c.hi) - row.m) - row.log_s) + 0.0);
+    t.lo = ~(uint32_t)(k * a.V + (int)~c.lo);
+  }
+  return t;
+}
+
+__device__ __forceinline__ void write_out(const BeamArgs& a, int b, int lane, const TotalKey& k) {
+  if (lane < a.width) {
+    const long long o = (long long)b * a.width + lane;
+    const uint32_t flat = ~k.lo;
+    a.out_scores[o] = k.hi ? (float)unordered(k.hi) : -INFINITY;
+    a.out_parent[o] = k.hi ? (int32_t)(flat / (uint32_t)a.V) : -1;
+    a.out_token[o] = k.hi ? (int32_t)(flat % (uint32_t)a.V) : -1;
+  }
+}
+
+// The wavefronts' lists, P lanes each and 64 / P to a wavefront: all joined in wavefront 0.
+template <int P>
+__device__ __forceinline__ void join_block(TotalKey& acc, TotalKey (*lds)[64], int wave, int waves, int lane) {
+  if constexpr (P <= 8) join<P>(acc, lane_xor<15>(acc), lane);
+  if constexpr (P <= 16) join<P>(acc, lane_xor<31>(acc), lane);
+  if constexpr (P <= 32) join<P>(acc, lane_xor<63>(acc), lane);
+  for (int half = waves >> 1; half >= 1; half >>= 1) {  // waves: a power of two
+    if (wave >= half && wave < 2 * half) lds[wave][lane] = acc;
+    __syncthreads();
+    if (wave < half) join<P>(acc, lds[wave + half][(lane & ~(P - 1)) | (P - 1 - (lane & (P - 1)))], lane);
+    __syncthreads();
+  }
+}
+
+// One launch for short rows: a block per utterance, its wavefronts share the beams.
+// 32 values a lane, with what they are loaded into, do not fit the 128 registers of 16 wavefronts: such blocks have 8.
+template <class T, int E, int P>
+__global__ __launch_bounds__(E == 32 ? 512 : 1024) void k_beam_rows(BeamArgs a) {
+  __shared__ RowKey lists[kMaxBeams][P];
+  __shared__ RowSum rows[kMaxBeams];
+  __shared__ TotalKey tree[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
+  RowKey* buf = reinterpret_cast<RowKey*>(tree[wave]);  // 128 keys; the lists are joined there after the barrier
+  for (int k = wave; k < a.K; k += waves) {
+    const float score = a.scores[(long long)b * a.K + k];
+    const bool done = a.finished && a.finished[(long long)b * a.K + k];
+    RowKey best = {0u, 0u};
+    RowSum row = {0.0, 0.0};
+    if (live_score(score) && !done) {  // uniform
+      float x[E], m;
+      double s;
+      load_piece<T, E>(a, b, k, 0, lane, x);
+      best = best_of_piece<E>(x, 0, a.width, lane, buf, &m, &s);
+      row = RowSum{(double)m, log(s)};
+      if (!(s > 0.0)) best = RowKey{0u, 0u};  // nothing allowed, or a NaN or +inf among the values
+    }
+    if (lane < P) lists[k][lane] = lane < a.width ? best : RowKey{0u, 0u};
+    if (lane == 0) rows[k] = row;
+  }
+  __syncthreads();
+  TotalKey acc = {0ull, 0u};
+  constexpr int G = 64 / P;
+  const int i = lane & (P - 1);
+  for (int k0 = wave * G; k0 < a.K; k0 += waves * G) {
+    const int k = k0 + lane / P;
+    TotalKey t = {0ull, 0u};
+    if (k < a.K) {
+      const float score = a.scores[(long long)b * a.K + k];
+      const bool done = a.finished && a.finished[(long long)b * a.K + k];
+      const int r = P - 1 - i;
+      if (live_score(score) && (!done || r == 0)) t = total_key(a, k, done, score, rows[k], lists[k][r]);
+    }
+    join<P>(acc, t, lane);
+  }
+  join_block<P>(acc, tree, wave, waves, lane);
+  if (wave == 0) write_out(a, b, lane, acc);
+}
+
+// Long rows, first launch: a wavefront per piece.  Workspace: the pieces' sums, then their lists of P keys.
+struct PieceSum {
+  double s;
+  float m, pad;
+};
+template <class T, int P>
+__global__ __launch_bounds__(256) void k_beam_pieces(BeamArgs a, PieceSum* sums, RowKey* lists) {
+  __shared__ RowKey buf[4][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long id = (long long)blockIdx.x * 4 + wave;
+  if (id >= (long long)a.B * a.K * a.pieces) return;
+  const int piece = (int)(id % a.pieces);
+  const long long row = id / a.pieces;
+  if (!live_score(a.scores[row]) || (a.finished && a.finished[row])) return;  // nothing of it is read
+  float x[kPiece / 64], m;
+  double s;
+  load_piece<T, kPiece / 64>(a, (int)(row / a.K), (int)(row % a.K), piece * kPiece, lane, x);
+  const RowKey best = best_of_piece<kPiece / 64>(x, piece * kPiece, a.width, lane, buf[wave], &m, &s);
+  if (lane < P) lists[id * P + lane] = lane < a.width ? best : RowKey{0u, 0u};
+  if (lane == 0) sums[id] = PieceSum{s, m, 0.f};
+}
+
+// Second launch: a block per utterance joins the pieces.
+template <int P>
+__global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* sums, const RowKey* lists) {
+  __shared__ RowSum rows[kMaxBeams];
+  __shared__ float live[kMaxBeams];  // the score of a beam that has candidates, else NaN
+  __shared__ TotalKey tree[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
+  for (int k = wave; k < a.K; k += waves) {
+    const long long row = (long long)b * a.K + k;
+    float score = a.scores[row];
+    const bool done = a.finished && a.finished[row];
+    RowSum of = {0.0, 0.0};
+    if (!live_score(score)) score = NAN;
+    else if (!done) {  // uniform
+      float m = -INFINITY;
+      for (int p = lane; p < a.pieces; p += 64) m = fmaxf(m, sums[row * a.pieces + p].m);
+      m = wave_max(m);
+      double s = 0.0;
+      for (int p = lane; p < a.pieces; p += 64) {
+        const PieceSum q = sums[row * a.pieces + p];
+        // a piece without an allowed symbol has m = -inf and s = 0; a NaN sum stays one
+        s += q.m == -INFINITY ? q.s : q.s * exp((double)q.m - (double)m);
+      }
+      s = wave_sum(s);
+      of = RowSum{(double)m, log(s)};
+      if (!(s > 0.0)) score = NAN;
+    }
+    if (lane == 0) {
+      rows[k] = of;
+      live[k] = score;
+    }
+  }
+  __syncthreads();
+  TotalKey acc = {0ull, 0u};
+  constexpr int G = 64 / P;
+  const int i = lane & (P - 1), r = P - 1 - i;
+  const int lists_here = a.K * a.pieces;
+  for (int l0 = wave * G; l0 < lists_here; l0 += waves * G) {
+    const int l = l0 + lane / P;
+    TotalKey t = {0ull, 0u};
+    if (l < lists_here) {
+      const int k = l / a.pieces, piece = l - k * a.pieces;
+      const float score = live[k];
+      const bool done = a.finished && a.finished[(long long)b * a.K + k];
+      if (score == score) {
+        if (done) {
+          if (piece == 0 && r == 0) t = total_key(a, k, true, score, rows[k], RowKey{0u, 0u});
+        } else {
+          t = total_key(a, k, false, score, rows[k], lists[((long long)b * lists_here + l) * P + r]);
+        }
+      }
+    }
+    if (__any(t > acc)) join<P>(acc, t, lane);  // lists that hold nothing better than the last of acc change nothing
+  }
+  join_block<P>(acc, tree, wave, waves, lane);
+  if (wave == 0) write_out(a, b, lane, acc);
+}
+
+int list_lanes(int width) { return width <= 8 ? 8 : width <= 16 ? 16 : width <= 32 ? 32 : 64; }
+int pieces_of(int V) { return V <= kPiece ? 0 : (V + kPiece - 1) / kPiece; }
+int pow2_up(int v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+
+template <class T, int P>
+int launch_select(const BeamArgs& a, void* workspace, hipStream_t st) {
+  if (a.pieces == 0) {
+    const int most = a.V <= 1024 ? 16 : 8, waves = a.K >= most ? most : pow2_up(a.K);
+    if (a.V <= 512) k_beam_rows<T, 8, P><<<a.B, waves * 64, 0, st>>>(a);
+    else if (a.V <= 1024) k_beam_rows<T, 16, P><<<a.B, waves * 64, 0, st>>>(a);
+    else k_beam_rows<T, 32, P><<<a.B, waves * 64, 0, st>>>(a);
+  } else {
+    const long long n = (long long)a.B * a.K * a.pieces;
+    PieceSum* sums = static_cast<PieceSum*>(workspace);
+    RowKey* lists = reinterpret_cast<RowKey*>(sums + n);
+    k_beam_pieces<T, P><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(a, sums, lists);
+    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
+    const int waves = min(16, pow2_up((a.K * a.pieces * P + 63) / 64));
+    k_beam_join<P><<<a.B, waves * 64, 0, st>>>(a, sums, lists);
+  }
+  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+}
+template <class T>
+int launch_select_width(const BeamArgs& a, void* workspace, hipStream_t st) {
+  switch (list_lanes(a.width)) {
+    case 8: return launch_select<T, 8>(a, workspace, st);
+    case 16: return launch_select<T, 16>(a, workspace, st);
+    case 32: return launch_select<T, 32>(a, workspace, st);
+  }
+  return launch_select<T, 64>(a, workspace, st);
+}
+
+int check_select(int B, int K, int V, int width) {
+  if (B < 1 || K < 1 || V < 1 || width < 1) return RNNT_MI355X_INVALID_VALUE;
+  if (K > kMaxBeams || width > kMaxWidth || (long long)K * V > 0x7fffffffll ||
+      (long long)B * K * ((V + kPiece - 1) / kPiece) > 0x7fffffffll)
+    return RNNT_MI355X_UNSUPPORTED_SIZE;
+  return RNNT_MI355X_OK;
+}
+
+// ---- states in their new order ------------------------------------------------------------------------------------------
+struct ReorderTensor {
+  const char* src;
+  char* dst;
+  long long outer_bytes, batch_bytes, beam_bytes;  // strides of src; dst is dense [outer, B, width, row]
+  long long row_bytes;
+  unsigned first, pieces;  // first work item of this tensor, work items a row
+};
+struct ReorderArgs {
+  ReorderTensor t[RNNT_MI355X_REORDER_MAX];
+  const int32_t* parent;
+  int n, B, K, width;
+};
+constexpr int kRowPiece = 4096;  // bytes of a row that one wavefront copies: four 16-byte loads a lane
+
+// A wavefront per piece of a row: bound by memory, or by the launch for the states of a single utterance; all tensors of a
+// step go in one launch.
+__global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a, unsigned items) {
+  const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (id >= items) return;
+  int n = 0;
+#pragma unroll
+  for (int i = 1; i < RNNT_MI355X_REORDER_MAX; ++i)
+    if (i < a.n && id >= a.t[i].first) n = i;
+  const ReorderTensor t = a.t[n];
+  const unsigned local = id - t.first, row = local / t.pieces, piece = local - row * t.pieces;
+  const unsigned bw = row % (unsigned)(a.B * a.width), outer = row / (unsigned)(a.B * a.width), b = bw / (unsigned)a.width;
+  const int parent = a.parent[bw];
+  const long long at = (long long)piece * kRowPiece;
+  const int n_bytes = (int)min((long long)kRowPiece, t.row_bytes - at);
+  char* d = t.dst + (long long)row * t.row_bytes + at;
+  const bool there = parent >= 0 && parent < a.K;
+  const char* s = t.src + outer * t.outer_bytes + b * t.batch_bytes + (there ? parent : 0) * t.beam_bytes + at;
+  u4 v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int o = (j * 64 + lane) * 16;
+    v[j] = u4{0u, 0u, 0u, 0u};
+    if (there && o + 16 <= n_bytes) v[j] = *reinterpret_cast<const u4_any*>(s + o);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int o = (j * 64 + lane) * 16;
+    if (o + 16 <= n_bytes) *reinterpret_cast<u4_any*>(d + o) = v[j];
+  }
+  const int tail = n_bytes & ~15;  // the last bytes of a row, one a lane
+  if (tail + lane < n_bytes) d[tail + lane] = there ? s[tail + lane] : 0;
+}
+
+}  // namespace
+
+extern "C" int rnnt_mi355x_beam_select_workspace_bytes(int B, int K, int V, int width, size_t* out_bytes) {
+  if (!out_bytes) return RNNT_MI355X_INVALID_VALUE;
+  const int rc = check_select(B, K, V, width);
+  if (rc != RNNT_MI355X_OK) return rc;
+  *out_bytes = (size_t)B * K * pieces_of(V) * (sizeof(PieceSum) + sizeof(RowKey) * list_lanes(width));
+  return RNNT_MI355X_OK;
+}
+
+extern "C" int rnnt_mi355x_beam_select(const void* logits, long long logits_batch_stride, long long logits_beam_stride, int dtype,
+                                       const void* enc, long long enc_batch_stride, const float* scores, const uint8_t* allowed,
+                                       long long allowed_batch_stride, const uint8_t* finished, int end, int B, int K, int V,
+                                       int width, float* out_scores, int32_t* out_parent, int32_t* out_token, void* workspace,
+                                       void* hip_stream) {
+  const int rc = check_select(B, K, V, width);
+  if (rc != RNNT_MI355X_OK) return rc;
+  if (!logits || !scores || !out_scores || !out_parent || !out_token || logits_batch_stride < 0 || logits_beam_stride < 0 ||
+      enc_batch_stride < 0 || allowed_batch_stride < 0 || (finished && (end < 0 || end >= V)) || (pieces_of(V) && !workspace))
+    return RNNT_MI355X_INVALID_VALUE;
+  BeamArgs a;
+  a.logits = logits;
+  a.enc = enc;
+  a.scores = scores;
+  a.allowed = allowed;
+  a.finished = finished;
+  a.logits_b = logits_batch_stride;
+  a.logits_k = logits_beam_stride;
+  a.enc_b = enc_batch_stride;
+  a.allowed_b = allowed_batch_stride;
+  a.B = B;
+  a.K = K;
+  a.V = V;
+  a.width = width;
+  a.end = end;
+  a.pieces = pieces_of(V);
+  a.out_scores = out_scores;
+  a.out_parent = out_parent;
+  a.out_token = out_token;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  switch (dtype) {
+    case RNNT_MI355X_FP32: return launch_select_width<Fp32>(a, workspace, st);
+    case RNNT_MI355X_BF16: return launch_select_width<Bf16>(a, workspace, st);
+    case RNNT_MI355X_FP16: return launch_select_width<Fp16>(a, workspace, st);
+  }
+  return RNNT_MI355X_INVALID_VALUE;
+}
+
+extern "C" int rnnt_mi355x_beam_reorder(const rnnt_mi355x_reorder_tensor* tensors, int n_tensors, const int32_t* parent, int B, int K,
+                                        int width, void* hip_stream) {
+  if (!tensors || !parent || n_tensors < 1 || B < 1 || K < 1 || width < 1) return RNNT_MI355X_INVALID_VALUE;
+  if (n_tensors > RNNT_MI355X_REORDER_MAX || (long long)B * width > 0x7fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
+  ReorderArgs a;
+  a.parent = parent;
+  a.n = n_tensors;
+  a.B = B;
+  a.K = K;
+  a.width = width;
+  long long items = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    const rnnt_mi355x_reorder_tensor& t = tensors[i];
+    if (!t.src || !t.dst || t.outer < 1 || t.row_bytes < 1 || t.outer_stride < 0 || t.batch_stride < 0 || t.beam_stride < 0)
+      return RNNT_MI355X_INVALID_VALUE;
+    const long long pieces = (t.row_bytes + kRowPiece - 1) / kRowPiece, rows = t.outer * B * width;
+    if (t.outer > 0x7fffffffll || rows > 0x7fffffffll || pieces > 0x7fffffffll || rows * pieces > 0x7fffffffll)
+      return RNNT_MI355X_UNSUPPORTED_SIZE;
+    a.t[i] = ReorderTensor{static_cast<const char*>(t.src), static_cast<char*>(t.dst), t.outer_stride, t.batch_stride, t.beam_stride,
+                           t.row_bytes, (unsigned)items, (unsigned)pieces};
+    items += rows * pieces;
+    if (items > 0x7fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
+  }
+  k_beam_reorder<<<(unsigned)((items + 3) / 4), 256, 0, static_cast<hipStream_t>(hip_stream)>>>(a, (unsigned)items);
+  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+}

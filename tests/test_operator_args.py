@@ -1,0 +1,105 @@
+"""Dropout and beam operators without a GPU: known answers of the generator's checker, refusals of the C entry points before
+any launch, refusals of the Python entry points."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import rnnt_amd
+from oracle import operators as orc
+from rnnt_amd import _lib, _operator
+
+ONE = 4096  # an address that is never dereferenced: validation fails first
+
+
+def test_philox_known_answers():
+    # the published vectors of Philox4x32-10: zeros, all ones, digits of pi
+    def words(c, k):
+        return [int(w) for w in orc.philox4x32(c, k)]
+    assert words((0, 0, 0, 0), (0, 0)) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    f = 0xFFFFFFFF
+    assert words((f, f, f, f), (f, f)) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert words((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0)) == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+
+
+def test_dropout_entry_point_refuses():
+    f = _lib.lib().rnnt_mi355x_dropout
+
+    def call(x=ONE, xs=8, y=2 * ONE, rows=4, cols=8, dtype=0, drop=100, seed=1, off=1):
+        return f(x, xs, y, rows, cols, dtype, drop, seed, off, None, None)
+    for bad in ({"x": None}, {"y": None}, {"rows": 0}, {"cols": 0}, {"xs": 7}, {"drop": -1}, {"drop": 65536}, {"dtype": 3}, {"dtype": -1},
+                {"x": ONE, "y": ONE, "xs": 9}):
+        assert call(**bad) == _lib.INVALID_VALUE, bad
+    assert call(rows=1 << 31) == _lib.UNSUPPORTED_SIZE
+    assert call(rows=(1 << 31) - 1, cols=1 << 20, xs=1 << 20) == _lib.UNSUPPORTED_SIZE
+
+
+def test_beam_select_entry_point_refuses():
+    L = _lib.lib()
+    n = ctypes.c_size_t(0)
+    q = L.rnnt_mi355x_beam_select_workspace_bytes
+    assert q(2, 4, 2048, 4, ctypes.byref(n)) == 0 and n.value == 0
+    assert q(2, 4, 2049, 4, ctypes.byref(n)) == 0 and n.value == 2 * 4 * 2 * (16 + 8 * 8)
+    assert q(2, 4, 2049, 33, ctypes.byref(n)) == 0 and n.value == 2 * 4 * 2 * (16 + 64 * 8)
+    assert q(2, 4, 2049, 4, None) == _lib.INVALID_VALUE
+    for bad in ((0, 4, 8, 4), (1, 0, 8, 4), (1, 4, 0, 4), (1, 4, 8, 0)):
+        assert q(*bad, ctypes.byref(n)) == _lib.INVALID_VALUE
+    for big in ((1, 65, 8, 4), (1, 4, 8, 65), (1, 64, 1 << 25, 4), (1 << 20, 64, 1 << 20, 4)):
+        assert q(*big, ctypes.byref(n)) == _lib.UNSUPPORTED_SIZE
+
+    def call(logits=ONE, sb=32, sk=8, dtype=0, scores=ONE, finished=None, end=0, B=2, K=4, V=8, width=4, o=ONE, ws=None):
+        return L.rnnt_mi355x_beam_select(logits, sb, sk, dtype, None, 0, scores, None, 0, finished, end, B, K, V, width, o, o, o, ws, None)
+    for bad in ({"logits": None}, {"scores": None}, {"o": None}, {"sb": -1}, {"sk": -8}, {"dtype": 5}, {"finished": ONE, "end": 8},
+                {"finished": ONE, "end": -1}, {"V": 3000, "sk": 3000, "ws": None}, {"width": 0}):
+        assert call(**bad) == _lib.INVALID_VALUE, bad
+    assert call(width=65) == _lib.UNSUPPORTED_SIZE
+
+
+def test_beam_reorder_entry_point_refuses():
+    f = _lib.lib().rnnt_mi355x_beam_reorder
+
+    def call(n=1, parent=ONE, B=2, K=3, W=4, **kw):
+        t = _lib.ReorderTensor(**{"src": ONE, "dst": 2 * ONE, "outer": 1, "outer_stride": 0, "batch_stride": 48, "beam_stride": 16, "row_bytes": 16, **kw})
+        return f((_lib.ReorderTensor * 17)(*[t] * 17), n, parent, B, K, W, None)
+    for bad in ({"n": 0}, {"parent": None}, {"B": 0}, {"K": 0}, {"W": 0}, {"src": None}, {"dst": None}, {"outer": 0}, {"row_bytes": 0},
+                {"outer_stride": -1}, {"batch_stride": -1}, {"beam_stride": -1}):
+        assert call(**bad) == _lib.INVALID_VALUE, bad
+    assert call(n=17) == _lib.UNSUPPORTED_SIZE
+    assert call(outer=1 << 31) == _lib.UNSUPPORTED_SIZE
+    assert call(row_bytes=1 << 44) == _lib.UNSUPPORTED_SIZE
+    assert f(None, 1, ONE, 1, 1, 1, None) == _lib.INVALID_VALUE
+
+
+def test_python_refusals_of_host_tensors():
+    x = torch.zeros(2, 3, 8)
+    with pytest.raises(ValueError, match="MI355X"):
+        rnnt_amd.dropout(x, 0.1)
+    with pytest.raises(ValueError, match="MI355X"):
+        rnnt_amd.beam_select(x, torch.zeros(2, 3), 2)
+    with pytest.raises(ValueError, match="MI355X"):
+        rnnt_amd.beam_reorder(torch.zeros(2, 2, dtype=torch.int32), [x])
+    with pytest.raises(TypeError):
+        rnnt_amd.dropout([1.0], 0.1)
+
+
+def test_rates_and_seeds():
+    assert _operator.drop16("d", 0.0) == 0 and _operator.drop16("d", 0.5) == 32768 and _operator.drop16("d", 1e-7) == 0
+    for bad in (-0.1, 1.0, 1.5, float("nan"), 1 - 2.0 ** -18):
+        with pytest.raises(ValueError):
+            _operator.drop16("d", bad)
+    cpu = torch.device("cpu")
+    assert _operator.seed_offset("d", 2 ** 64 - 1, 7, cpu) == (2 ** 64 - 1, 7, None)
+    for seed, off in ((-1, 0), (2 ** 64, 0), (0, -1), (0, 2 ** 64), (0, torch.zeros(1)), (0, torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            _operator.seed_offset("d", seed, off, cpu)
+    t = torch.zeros(1, dtype=torch.int64)
+    assert _operator.seed_offset("d", 3, t, cpu) == (3, 0, t)
+
+
+def test_checker_of_the_mask_keeps_the_right_share():
+    s = orc.dropout_scale(400, 501, 0.3, 5, 9)
+    n = s.size
+    kept = (s > 0).sum()
+    assert abs(kept - 0.7 * n) < 5 * np.sqrt(n * 0.21)
+    assert np.allclose(s[s > 0], 1 / 0.7, rtol=1e-4)
