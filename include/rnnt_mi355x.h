@@ -240,7 +240,7 @@ int rnnt_mi355x_joint_log_softmax(const float* f, int f_rows, const float* g, in
                                   const int32_t* g_index, int n_rows, int V, float* out, int32_t* bad_index_flag,
                                   void* hip_stream);
 
-/* ---- operators around the joint network: dropout, beam step ----------------------
+/* ---- operators around the joint network: dropout, Dense layer, beam step -----------
  * They take float32, bfloat16 and float16 tensors (`dtype`); every sum, softmax statistic
  * and score is held in 32 bits or more. */
 #define RNNT_MI355X_FP32 0
@@ -258,6 +258,44 @@ int rnnt_mi355x_joint_log_softmax(const float* f, int f_rows, const float* g, in
  * replay when the caller advances it. */
 int rnnt_mi355x_dropout(const void* x, long long x_stride, void* y, long long rows, int cols, int dtype, int drop16,
                         uint64_t seed, uint64_t offset, const uint64_t* offset_dev, void* hip_stream);
+
+/* Dense layer of any width with its epilogue (TimeDistributed(Dense) and Dropout of
+ * get_fc, reference rnnt/keras_model.py:83-104; rnnt_mi355x_dense_* above are its
+ * float32 special case for widths up to 128):
+ *   z = x kernel + bias,  y = residual + dropout(act(z))
+ *   dz = dropout'(dy) act'(z), dx = dz kernel^T, dkernel = x^T dz, dbias = sum over rows of dz
+ * (d residual is dy).  x: [rows, in], kernel: [in, out] (Keras), residual, y, aux,
+ * dy: [rows, out]; all of one `dtype`, last dimension contiguous, rows *_stride elements
+ * apart (y and aux dense).  float32 products are accurate to float32 rounding (three
+ * bfloat16 parts an operand), sums are float32.  bias, residual and aux may be NULL.
+ * act: RNNT_MI355X_ACT_*; gelu is the exact z Phi(z).  Dropout as rnnt_mi355x_dropout
+ * draws it for [rows, out] (drop16 0: none).
+ * The backward pass takes the same layer and needs, unless act is linear, aux as the
+ * forward pass wrote it: the pre-activation, float32 for float32 and float16 layers,
+ * float16 for bfloat16 ones.  Without residual, relu layers and float32 tanh layers may
+ * go without it (aux NULL in both passes); y is read instead.  dx, dkernel, dbias may
+ * be NULL.  Sums run in a fixed order: equal calls give equal bits.
+ * Workspace: the sizes rnnt_mi355x_layer_workspace_bytes gives for the very pointers
+ * and strides (their alignment decides the kernels); forward 0: may be NULL.  y may be
+ * residual itself when its stride is `out`.  rows < 2^31 - 2^16, in, out <= 2^24. */
+#define RNNT_MI355X_ACT_LINEAR 0
+#define RNNT_MI355X_ACT_TANH 1
+#define RNNT_MI355X_ACT_RELU 2
+#define RNNT_MI355X_ACT_GELU 3
+#define RNNT_MI355X_ACT_SILU 4
+typedef struct {
+  const void *x, *kernel, *bias, *residual;
+  void *y, *aux;
+  long long x_stride, kernel_stride, residual_stride, rows;
+  int in, out, dtype, act, drop16;
+  uint64_t seed, offset;
+  const uint64_t* offset_dev;
+} rnnt_mi355x_layer;
+int rnnt_mi355x_layer_workspace_bytes(const rnnt_mi355x_layer* layer, const void* dy, long long dy_stride,
+                                      size_t* forward_bytes, size_t* backward_bytes);
+int rnnt_mi355x_layer_forward(const rnnt_mi355x_layer* layer, void* workspace, void* hip_stream);
+int rnnt_mi355x_layer_backward(const rnnt_mi355x_layer* layer, const void* dy, long long dy_stride, void* dx, void* dkernel,
+                               void* dbias, void* workspace, void* hip_stream);
 
 /* One step of a beam search (what reference rnnt/rnnt_decoder.py:95-233 does with the
  * log-probabilities of its inner step).  logits: [B, K, V] (last dimension

@@ -50,6 +50,14 @@ class ReorderTensor(ctypes.Structure):
     _fields_ = [("src", _vp), ("dst", _vp)] + [(n, _ll) for n in ("outer", "outer_stride", "batch_stride", "beam_stride", "row_bytes")]
 
 
+class Layer(ctypes.Structure):
+    """rnnt_mi355x_layer (`in` and `out` there)"""
+    _fields_ = ([(n, _vp) for n in ("x", "kernel", "bias", "residual", "y", "aux")]
+                + [(n, _ll) for n in ("x_stride", "kernel_stride", "residual_stride", "rows")]
+                + [(n, _i) for n in ("n_in", "n_out", "dtype", "act", "drop16")]
+                + [("seed", _u64), ("offset", _u64), ("offset_dev", _vp)])
+
+
 _SIGNATURES = {
     "rnnt_mi355x_workspace_bytes": (ctypes.c_int, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "rnnt_mi355x_forward": (ctypes.c_int, [_vp] * 4 + _META + [_vp, _vp, _vp]),
@@ -76,6 +84,9 @@ _SIGNATURES = {
     "rnnt_mi355x_dense_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "rnnt_mi355x_joint_log_softmax": (ctypes.c_int, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "rnnt_mi355x_dropout": (ctypes.c_int, [_vp, _ll, _vp, _ll, _i, _i, _i, _u64, _u64, _vp, _vp]),
+    "rnnt_mi355x_layer_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Layer), _vp, _ll, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "rnnt_mi355x_layer_forward": (ctypes.c_int, [ctypes.POINTER(Layer), _vp, _vp]),
+    "rnnt_mi355x_layer_backward": (ctypes.c_int, [ctypes.POINTER(Layer), _vp, _ll] + [_vp] * 5),
     "rnnt_mi355x_beam_select_workspace_bytes": (ctypes.c_int, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "rnnt_mi355x_beam_select": (ctypes.c_int, [_vp, _ll, _ll, _i, _vp, _ll, _vp, _vp, _ll, _vp] + [_i] * 5 + [_vp] * 5),
     "rnnt_mi355x_beam_reorder": (ctypes.c_int, [ctypes.POINTER(ReorderTensor), _i, _vp, _i, _i, _i, _vp]),

@@ -14,8 +14,8 @@ CSRC = os.path.join(_HERE, "csrc")
 SOURCES = [os.path.join(CSRC, "rnnt_mi355x.hip"), os.path.join(CSRC, "fc_joint.hip"),
            os.path.join(CSRC, "skinny_dense.hip"), os.path.join(CSRC, "decode_step.hip")]
 # operators around the joint network
-OPERATOR_SOURCES = [os.path.join(CSRC, "dropout.hip"), os.path.join(CSRC, "beam.hip")]
-OPERATOR_PIECES = [os.path.join(CSRC, "op_util.h")]
+OPERATOR_SOURCES = [os.path.join(CSRC, n) for n in ("dropout.hip", "beam.hip", "layer.hip", "layer_fp32.hip", "layer_bf16.hip", "layer_fp16.hip")]
+OPERATOR_PIECES = [os.path.join(CSRC, n) for n in ("op_util.h", "layer_plan.h", "layer_gemm.h", "layer_gemm_launch.h")]
 # rnnt_mi355x.hip is one translation unit whose kernels live in these included pieces
 PIECES = [os.path.join(CSRC, n) for n in ("workspace.h", "device_util.h", "lse_rows.h", "sweep.h", "grad_rows.h", "grad_span.h", "grad_split.h", "cell_coef.h", "grad_flat.h", "lse_span.h",
                                           "small_vocab.h", "joint.h", "aux_kernels.h")]

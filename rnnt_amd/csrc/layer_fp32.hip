@@ -1,0 +1,6 @@
+// The Dense layer's matrix products in fp32 (kernels: layer_gemm.h).
+#include "layer_gemm_launch.h"
+
+int layer_gemm_fp32(int product, int block, bool, const void* args, hipStream_t st) {
+  return launch_product<Fp32, false>(product, block, *static_cast<const GemmArgs*>(args), st);
+}

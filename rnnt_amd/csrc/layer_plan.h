@@ -1,0 +1,14 @@
+// How a Dense layer's products are cut into blocks, shared by the host code (layer.hip) and the kernels of each type.
+#pragma once
+#include <hip/hip_runtime.h>
+
+// the three products of a layer: which operand is strided along k
+enum LayerProduct { kForward = 0 /* x k-fast, W k-slow */, kInputGrad = 1 /* dz, W k-fast */, kKernelGrad = 2 /* x, dz k-slow */ };
+// block of the result
+enum LayerBlock { kBlock32x128 = 0, kBlock64x64 = 1, kBlock128x128 = 2, kBlock256x256 = 3 };
+
+// launch one product; `args` is a GemmArgs (layer_gemm.h), every translation unit has its own copy of that type
+#define RNNT_HIDDEN __attribute__((visibility("hidden")))
+RNNT_HIDDEN int layer_gemm_fp32(int product, int block, bool direct, const void* args, hipStream_t st);
+RNNT_HIDDEN int layer_gemm_bf16(int product, int block, bool direct, const void* args, hipStream_t st);
+RNNT_HIDDEN int layer_gemm_fp16(int product, int block, bool direct, const void* args, hipStream_t st);

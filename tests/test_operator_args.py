@@ -71,6 +71,40 @@ def test_beam_reorder_entry_point_refuses():
     assert f(None, 1, ONE, 1, 1, 1, None) == _lib.INVALID_VALUE
 
 
+def _layer(**kw):
+    return _lib.Layer(**{"x": ONE, "kernel": 2 * ONE, "y": 3 * ONE, "x_stride": 8, "kernel_stride": 6, "rows": 4, "n_in": 8, "n_out": 6, **kw})
+
+
+def test_layer_entry_points_refuse():
+    L = _lib.lib()
+    f, b, q = L.rnnt_mi355x_layer_forward, L.rnnt_mi355x_layer_backward, L.rnnt_mi355x_layer_workspace_bytes
+    for bad in ({"x": None}, {"kernel": None}, {"y": None}, {"rows": 0}, {"n_in": 0}, {"n_out": 0}, {"x_stride": 7}, {"kernel_stride": 5}, {"dtype": 3},
+                {"dtype": -1}, {"act": 5}, {"act": -1}, {"drop16": -1}, {"drop16": 65536}, {"residual": ONE, "residual_stride": 5}):
+        assert f(_layer(**bad), None, None) == _lib.INVALID_VALUE, bad
+    for big in ({"rows": 1 << 31}, {"n_in": (1 << 24) + 1, "x_stride": 1 << 25}, {"n_out": (1 << 24) + 1, "kernel_stride": 1 << 25}):
+        assert f(_layer(**big), None, None) == _lib.UNSUPPORTED_SIZE, big
+    assert f(None, None, None) == _lib.INVALID_VALUE
+    assert f(_layer(n_in=4000, x_stride=4000), None, None) == _lib.INVALID_VALUE  # split along k: needs its workspace
+
+    def back(layer, dy=ONE, stride=6, ws=ONE):
+        return b(layer, dy, stride, ONE, ONE, ONE, ws, None)
+    assert back(_layer(), dy=None) == back(_layer(), stride=5) == back(_layer(), ws=None) == back(_layer(x=None)) == _lib.INVALID_VALUE
+    # without the pre-activation only what y determines is accepted
+    for bad in ({"act": 3}, {"act": 4}, {"act": 1, "dtype": 1}, {"act": 1, "residual": ONE, "residual_stride": 6}, {"act": 2, "residual": ONE, "residual_stride": 6},
+                {"act": 2, "y": None}):
+        assert back(_layer(**bad)) == _lib.INVALID_VALUE, bad
+    n, m = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert q(_layer(), ONE, 6, ctypes.byref(n), ctypes.byref(m)) == 0 and n.value == 0 and m.value >= 24
+    assert q(_layer(n_in=4000, x_stride=4000), None, 0, ctypes.byref(n), None) == 0 and n.value > 0 and n.value % (4 * 6 * 4) == 0
+    assert q(_layer(), ONE, 5, None, ctypes.byref(m)) == _lib.INVALID_VALUE
+    assert q(None, None, 0, ctypes.byref(n), None) == _lib.INVALID_VALUE
+
+
+def test_layer_structure_has_the_size_of_the_header():
+    assert ctypes.sizeof(_lib.Layer) == 6 * 8 + 4 * 8 + 5 * 4 + 4 + 3 * 8
+    assert ctypes.sizeof(_lib.ReorderTensor) == 7 * 8
+
+
 def test_python_refusals_of_host_tensors():
     x = torch.zeros(2, 3, 8)
     with pytest.raises(ValueError, match="MI355X"):
@@ -79,6 +113,8 @@ def test_python_refusals_of_host_tensors():
         rnnt_amd.beam_select(x, torch.zeros(2, 3), 2)
     with pytest.raises(ValueError, match="MI355X"):
         rnnt_amd.beam_reorder(torch.zeros(2, 2, dtype=torch.int32), [x])
+    with pytest.raises(ValueError, match="MI355X"):
+        rnnt_amd.dense(x, torch.zeros(8, 4))
     with pytest.raises(TypeError):
         rnnt_amd.dropout([1.0], 0.1)
 
