@@ -17,7 +17,7 @@ struct DzArgs {
   const void *dy, *saved;
   void* dz;         // nullable: dz is dy (linear, no dropout) and only the sums are wanted
   float* partial;   // nullable [row blocks][N]
-  long long dy_ld;
+  long long dy_ld, dz_ld;
   int M, N, rows;   // rows of a block
   int act, from;
   DropArgs drop;
@@ -32,8 +32,24 @@ __device__ __forceinline__ void slopes8(const DzArgs& a, long long m, int n0, in
     const typename A::elem* p = static_cast<const typename A::elem*>(a.saved) + m * a.N + n0;
     if (n >= 8) unpack8<A>(load8_raw<A>(p), s);
     else load_some<A>(p, n, s);
+    switch (a.act) {
+      case kTanh:
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= slope_of(s[i], a.act);
+        for (int i = 0; i < 8; ++i) v[i] *= slope_of(s[i], kTanh);
+        break;
+      case kRelu:
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= slope_of(s[i], kRelu);
+        break;
+      case kGelu:
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= slope_of(s[i], kGelu);
+        break;
+      case kSilu:
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= slope_of(s[i], kSilu);
+        break;
+    }
   } else {  // y = act(z) * scale (0 where dropped: dy is dropped there as well)
     const typename T::elem* p = static_cast<const typename T::elem*>(a.saved) + m * a.N + n0;
     if (n >= 8) unpack8<T>(load8_raw<T>(p), s);
@@ -60,13 +76,13 @@ __global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a) {
 #pragma unroll 2
     for (int m = m0 + ty; m < m1; m += kDzLanes) {
       float v[8];
-      const typename T::elem* p = static_cast<const typename T::elem*>(a.dy) + m * a.dy_ld + n0;
+      const typename T::elem* p = static_cast<const typename T::elem*>(a.dy) + (long long)m * a.dy_ld + n0;
       if (left >= 8) unpack8<T>(load8_raw<T>(p), v);
       else load_some<T>(p, left, v);
       if (a.act != kLinear) slopes8<T>(a, m, n0, left, v);
       if (a.drop.drop) drop8(a.drop, (uint32_t)m, (uint32_t)n0 >> 3, v);
       if (a.dz) {
-        typename T::elem* q = static_cast<typename T::elem*>(a.dz) + (long long)m * a.N + n0;
+        typename T::elem* q = static_cast<typename T::elem*>(a.dz) + m * a.dz_ld + n0;
         if (left >= 8) store8<T>(q, v);
         else store_some<T>(q, left, v);
       }
@@ -93,8 +109,10 @@ __global__ __launch_bounds__(1024) void k_layer_db(const float* partial, int blo
   __shared__ float sums[16][64];
   const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
   float s = 0.f;
-  if (n < N)
+  if (n < N) {
+#pragma unroll 8
     for (int i = r; i < blocks; i += 16) s += partial[(long long)i * N + n];
+  }
   sums[r][c] = s;
   __syncthreads();
   if (r == 0 && n < N) {
@@ -105,64 +123,84 @@ __global__ __launch_bounds__(1024) void k_layer_db(const float* partial, int blo
 }
 
 // ---- joining the splits of a product -------------------------------------------------------------------------------------
+// A block takes 32 groups of eight columns of one tile's rows; 8 lanes share a group's splits.  The order is fixed.
 template <class T>
-__global__ __launch_bounds__(256) void k_layer_join(GemmArgs g) {
-  const int groups = (g.N + 7) / 8;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, m = id / groups;
-  if (m >= g.M) return;
-  const int n = (int)(id - m * groups) * 8, left = g.N - n;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const float* p = g.partial + m * g.N + n;
+__global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn) {
+  __shared__ float sums[8][32][9];
+  const int c = threadIdx.x & 31, s0 = threadIdx.x >> 5, groups = bn / 8, per_tile = bm * groups / 32;
+  const int tile = blockIdx.x / per_tile, group = (blockIdx.x - tile * per_tile) * 32 + c;
+  int tm, tn;
+  place_of(g, g.whole + tile, tm, tn);
+  const long long m = (long long)tm * bm + group / groups;
+  const int n = tn * bn + 8 * (group % groups), left = g.N - n;
+  const bool in = m < g.M && left > 0;
+  float v[1][8] = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+  if (in) {
+    const float* p = g.partial + (long long)tile * g.splits * bm * bn + 8 * group;
 #pragma unroll 4
-  for (int s = 0; s < g.splits; ++s, p += (long long)g.M * g.N) {
-    float w[8];
-    if (left >= 8) unpack8<Fp32>(load8_raw<Fp32>(p), w);
-    else load_some<Fp32>(p, left, w);
+    for (int s = s0; s < g.splits; s += 8) {
+      float w[8];
+      unpack8<Fp32>(load8_raw<Fp32>(p + (long long)s * bm * bn), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += w[i];
+      for (int i = 0; i < 8; ++i) v[0][i] += w[i];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[s0][c][i] = v[0][i];
+  __syncthreads();
+  if (s0 != 0 || !in) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int s = 1; s < 8; ++s) v[0][i] += sums[s][c][i];
   DropArgs drop = g.e.drop;
   if (drop.drop) load_offset(drop);
-  finish8<T>(g.e, drop, m, n, left, v);
+  finish<T, 1>(g.e, drop, {m}, g.M, n, left, v);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 struct Plan {
-  int block, splits, k_each, tiles_m, tiles_n;
+  int block, bm, bn, tiles_m, tiles_n, whole, splits, k_each;
   bool direct;
   size_t partial_bytes;
 };
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Which block, and in how many pieces along k.  256 CUs want two blocks of 128x128 each, and one of 256x256.
+constexpr int kCUs = 256;
+
+// Which block, and which tiles are cut along k.
 Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
   Plan p;
   p.direct = direct;
-  const int bk = dtype == RNNT_MI355X_FP32 ? 32 : 64;
-  int bm = 128, bn = 128;
+  p.bm = p.bn = 128;
   p.block = kBlock128x128;
+  const int steps = ceil_div(K, 32);
   if (product != kKernelGrad && M <= 32) {
-    p.block = kBlock32x128;
-    bm = 32;
+    p.block = kBlock32;
+    p.bm = 32;
+    p.bn = direct ? 64 : 128;
   } else if (M <= 64 || N <= 64) {
     p.block = kBlock64x64;
-    bm = bn = 64;
+    p.bm = p.bn = 64;
   } else if (direct && (long long)ceil_div(M, 256) * ceil_div(N, 256) * (product == kKernelGrad ? ceil_div(K, 4096) : 1) >= 192) {
     p.block = kBlock256x256;
-    bm = bn = 256;
+    p.bm = p.bn = 256;
   }
-  p.tiles_m = ceil_div(M, bm);
-  p.tiles_n = ceil_div(N, bn);
+  p.tiles_m = ceil_div(M, p.bm);
+  p.tiles_n = ceil_div(N, p.bn);
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
-  const int want = p.block == kBlock256x256 ? 256 : 512;
-  int splits = tiles >= want / 2 ? 1 : (int)(want / tiles);
-  const int most = K / (4 * bk);  // a piece has at least four steps
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  p.k_each = ceil_div(ceil_div(K, splits), 64) * 64;
+  // Rounds of one tile a CU are done whole.  The rest would leave CUs idle for a round: it is cut along k until there are
+  // two pieces for every CU (one of the largest block), each of four steps of 32 k at least.
+  const int want = p.block == kBlock256x256 ? kCUs : 2 * kCUs;
+  const int others = (int)(tiles % kCUs);
+  p.splits = others == 0 ? 1 : want / others;
+  if (p.splits > steps / 4) p.splits = steps / 4;
+  if (tiles > 16 * kCUs || p.splits < 2) p.splits = 1;
+  p.k_each = ceil_div(ceil_div(K, p.splits), 64) * 64;
   p.splits = ceil_div(K, p.k_each);
-  p.partial_bytes = p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  p.whole = (int)(p.splits == 1 ? tiles : tiles - others);
+  p.partial_bytes = (size_t)(tiles - p.whole) * p.splits * p.bm * p.bn * sizeof(float);
   return p;
 }
 
@@ -193,15 +231,15 @@ int run_product(int product, const Plan& p, const void* a, long long a_ld, const
   g.K = K;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
+  g.whole = p.whole;
   g.splits = p.splits;
   g.k_each = p.k_each;
   g.partial = partial;
   g.e = e;
-  if ((long long)p.tiles_m * p.tiles_n * p.splits > 0x7fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
   const int rc = gemm_of<T>(product, p.block, p.direct, g, st);
-  if (rc != RNNT_MI355X_OK || p.splits == 1) return rc;
-  const long long groups = (long long)M * ((N + 7) / 8);
-  k_layer_join<T><<<(unsigned)((groups + 255) / 256), 256, 0, st>>>(g);
+  const int others = p.tiles_m * p.tiles_n - p.whole;
+  if (rc != RNNT_MI355X_OK || others == 0) return rc;
+  k_layer_join<T><<<(unsigned)others * (p.bm * p.bn / 256), 256, 0, st>>>(g, p.bm, p.bn);
   return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
 }
 
@@ -222,7 +260,9 @@ int check_layer(const rnnt_mi355x_layer* l) {
       l->drop16 < 0 || l->drop16 > 65535 || l->x_stride < l->in || l->kernel_stride < l->out)
     return RNNT_MI355X_INVALID_VALUE;
   // 32-bit indexes inside an operand's rows and of its tiles
-  if (l->rows > 0x7fff0000ll || l->in > (1 << 24) || l->out > (1 << 24)) return RNNT_MI355X_UNSUPPORTED_SIZE;
+  if (l->rows > 0x7fff0000ll || l->in > (1 << 24) || l->out > (1 << 24) || ((l->rows + 63) / 64) * ((l->in + 63) / 64) > 0x7fffffffll ||
+      ((l->rows + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll)
+    return RNNT_MI355X_UNSUPPORTED_SIZE;
   return RNNT_MI355X_OK;
 }
 
@@ -236,6 +276,13 @@ int saved_by(const rnnt_mi355x_layer* l) {
 // row blocks of the dz pass: at most 1024 partial sums a column
 int dz_rows(long long M) { return M <= 65536 ? 64 : (int)((M + 1023) / 1024 + 7) / 8 * 8; }
 
+// dz's rows in the workspace.  Rows a multiple of 4 KiB apart put the same piece of all rows of a tile into the same few
+// memory channels: 32768 x 4096 x 1024 in bfloat16 ran 300 us with such rows and 257 us with rows 128 bytes longer.
+long long dz_stride(int out, int dtype) {
+  const long long e = dtype == RNNT_MI355X_FP32 ? 4 : 2;
+  return out * e % 4096 == 0 ? out + 128 / e : out;
+}
+
 struct BackwardPlan {
   bool need_dz;  // else dz is dy
   size_t dz_at, sums_at, partial_at, bytes;
@@ -247,9 +294,9 @@ BackwardPlan plan_backward(const rnnt_mi355x_layer* l, const void* dy, long long
   const size_t e = l->dtype == RNNT_MI355X_FP32 ? 4 : 2;
   b.need_dz = l->act != kLinear || l->drop16 != 0;
   b.dz_at = 0;
-  b.sums_at = align_up(b.need_dz ? (size_t)M * l->out * e : 0);
+  b.sums_at = align_up(b.need_dz ? (size_t)M * dz_stride(l->out, l->dtype) * e : 0);
   b.partial_at = b.sums_at + align_up((size_t)ceil_div(M, dz_rows(M)) * l->out * sizeof(float));
-  // dz lies in the workspace (256-byte boundaries), rows `out` apart
+  // dz lies in the workspace, on a 256-byte boundary
   const bool dz_direct = b.need_dz ? l->dtype != RNNT_MI355X_FP32 && l->out % 8 == 0 && l->out < (1 << 21) : can_go_direct(dy, dy_stride, l->out, l->dtype);
   b.dx = plan_product(kInputGrad, l->dtype, M, l->in, l->out, dz_direct && can_go_direct(l->kernel, l->kernel_stride, l->out, l->dtype));
   b.dk = plan_product(kKernelGrad, l->dtype, l->in, l->out, M, dz_direct && can_go_direct(l->x, l->x_stride, l->in, l->dtype));
@@ -281,7 +328,7 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
   const int M = (int)l->rows;
   char* ws = static_cast<char*>(workspace);
   const void* dz = b.need_dz ? ws + b.dz_at : dy;
-  const long long dz_ld = b.need_dz ? l->out : dy_stride;
+  const long long dz_ld = b.need_dz ? dz_stride(l->out, l->dtype) : dy_stride;
   float *sums = reinterpret_cast<float*>(ws + b.sums_at), *partial = reinterpret_cast<float*>(ws + b.partial_at);
   const int blocks = ceil_div(M, dz_rows(M));
   if (b.need_dz || dbias) {
@@ -291,6 +338,7 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
     a.dz = b.need_dz ? ws + b.dz_at : nullptr;
     a.partial = dbias ? sums : nullptr;
     a.dy_ld = dy_stride;
+    a.dz_ld = dz_ld;
     a.M = M;
     a.N = l->out;
     a.rows = dz_rows(M);

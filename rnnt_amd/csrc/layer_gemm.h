@@ -55,6 +55,7 @@ __device__ __forceinline__ float normal_of(float z, float& e) {
   const float tail = 0.5f * q * e;  // 1 - Phi(|z|)
   return z < 0.f ? tail : 1.f - tail;
 }
+__device__ __forceinline__ float floor_of(float z, float least) { return __builtin_elementwise_maximum(z, least); }  // NaN stays
 __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
     case kTanh: return tanh_of(z);
@@ -62,9 +63,9 @@ __device__ __forceinline__ float act_of(float z, int act) {
     case kGelu: {
       float e;
       const float p = normal_of(z, e);
-      return z == -INFINITY ? 0.f : z * p;
+      return floor_of(z, -64.f) * p;  // p = 0 there, and 0 times -inf would be NaN
     }
-    case kSilu: return z == -INFINITY ? 0.f : z * sigmoid_of(z);
+    case kSilu: return floor_of(z, -256.f) * sigmoid_of(z);
   }
   return z;
 }
@@ -91,58 +92,104 @@ __device__ __forceinline__ float slope_of(float z, int act) {
 }
 
 // The pre-activation that the backward pass reads: float32 for float32 and float16 layers, float16 for bfloat16 ones.
-// bfloat16 would put a rounding of 2^-9 into act'(z) on top of dz's own; float16 has 2^-12, at the same size.  Its range is
-// 2^-24 .. 65504: beyond it act' is at its limits, and below it only the sign of z counts.
+// bfloat16 would put a rounding of 2^-8 into act'(z) on top of dz's own; float16 has 2^-11, at the same size.  Past its
+// range it is infinite, where act' is at its limits; below it only relu's slope asks for more than z = 0 says, and relu
+// keeps its slope in the place of z.
 template <class T>
 struct AuxOf { using type = Fp32; };
 template <>
 struct AuxOf<Bf16> { using type = Fp16; };
-template <class T>
-__device__ __forceinline__ float aux_value(float z) {
-  if constexpr (T::code != RNNT_MI355X_BF16) return z;
-  // fminf / fmaxf drop NaN, which has to stay
-  const float c = z != z ? z : fminf(fmaxf(z, -65504.f), 65504.f);
-  return fabsf(c) < 5.9604645e-8f && c != 0.f ? copysignf(5.9604645e-8f, c) : c;
+
+// act(z) of eight values; the choice is the same for all lanes and made once.
+__device__ __forceinline__ void act8(int act, float (&v)[8]) {
+  switch (act) {
+    case kTanh:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], kTanh);
+      break;
+    case kRelu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], kRelu);
+      break;
+    case kGelu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], kGelu);
+      break;
+    case kSilu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], kSilu);
+      break;
+  }
 }
 
-// Eight consecutive results of a row, n of them inside it.
 template <class T>
-__device__ __forceinline__ void finish8(const Epilogue& e, const DropArgs& drop, long long m, int n0, int n, float (&v)[8]) {
+__device__ __forceinline__ Raw8<T> load_group(const typename T::elem* p, int n) {
+  if (n >= 8) return load8_raw<T>(p);
+  typename T::elem some[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) some[i] = i < n ? p[i] : 0;
+  Raw8<T> r;
+  __builtin_memcpy(&r, some, sizeof(some));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void store_group(typename T::elem* p, int n, const float (&v)[8]) {
+  if (n >= 8) store8<T>(p, v);
+  else store_some<T>(p, n, v);
+}
+
+// G times eight consecutive results, of rows m[g] and the same columns n0 .., n of them inside the row.  Stage by stage over
+// all G: a group's chain of the generator or of an activation is long, several of them fill each other's waits.
+template <class T, int G>
+__device__ __forceinline__ void finish(const Epilogue& e, const DropArgs& drop, const long long (&m)[G], int M, int n0, int n, float (&v)[G][8]) {
   using E = typename T::elem;
-  const bool full = n >= 8;
+  Raw8<T> res[G];
+  if (e.residual) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (m[g] < M) res[g] = load_group<T>(static_cast<const E*>(e.residual) + m[g] * e.residual_ld + n0, n);
+  }
   if (e.bias) {
     float b[8];
-    const E* p = static_cast<const E*>(e.bias) + n0;
-    if (full) unpack8<T>(load8_raw<T>(p), b);
-    else load_some<T>(p, n, b);
+    unpack8<T>(load_group<T>(static_cast<const E*>(e.bias) + n0, n), b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += b[i];
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[g][i] += b[i];
   }
   if (e.aux) {
     using A = typename AuxOf<T>::type;
-    float z[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = aux_value<T>(v[i]);
-    typename A::elem* p = static_cast<typename A::elem*>(e.aux) + m * e.out_ld + n0;
-    if (full) store8<A>(p, z);
-    else store_some<A>(p, n, z);
+    for (int g = 0; g < G; ++g) {
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = v[g][i];
+      if (e.act == kRelu) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = z[i] > 0.f ? 1.f : z[i];
+      }
+      if (m[g] < M) store_group<A>(static_cast<typename A::elem*>(e.aux) + m[g] * e.out_ld + n0, n, z);
+    }
   }
   if (e.act != kLinear) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], e.act);
+    for (int g = 0; g < G; ++g) act8(e.act, v[g]);
   }
-  if (drop.drop) drop8(drop, (uint32_t)m, (uint32_t)n0 >> 3, v);
-  if (e.residual) {
-    float r[8];
-    const E* p = static_cast<const E*>(e.residual) + m * e.residual_ld + n0;
-    if (full) unpack8<T>(load8_raw<T>(p), r);
-    else load_some<T>(p, n, r);
+  if (drop.drop) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
+    for (int g = 0; g < G; ++g) drop8(drop, (uint32_t)m[g], (uint32_t)n0 >> 3, v[g]);
   }
-  E* p = static_cast<E*>(e.out) + m * e.out_ld + n0;
-  if (full) store8<T>(p, v);
-  else store_some<T>(p, n, v);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (m[g] >= M) continue;
+    if (e.residual) {
+      float r[8];
+      unpack8<T>(res[g], r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[g][i] += r[i];
+    }
+    store_group<T>(static_cast<E*>(e.out) + m[g] * e.out_ld + n0, n, v[g]);
+  }
 }
 
 // ---- staging ------------------------------------------------------------------------------------------------------------
@@ -154,7 +201,7 @@ __device__ __forceinline__ void split8(const float (&v)[8], u4 (&q)[3]) {
     float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      const uint32_t ha = float_to_bf16_bits(a), hb = float_to_bf16_bits(b), w = ha | (hb << 16);
+      const uint32_t w = pack_bf16(a, b);
       q[p][i] = w;
       a -= __uint_as_float(w << 16);
       b -= __uint_as_float(w & 0xffff0000u);
@@ -171,9 +218,12 @@ struct Tile {
   static constexpr int kPlaneBytes = R * BK * 2, kBytes = kPlaneBytes * kPlanes<T>;
   static_assert(kPieces % THREADS == 0 && (!KS || R >= 64) && (BK == 32 || BK == 64), "tile shape");
 
-  // place p holds row p / kRow and piece (p % kRow) ^ permute(row): k-fast reads take one piece of 8 consecutive rows
-  // together, k-slow reads 32 bytes of 4 consecutive k
-  static __device__ __forceinline__ int permute(int row) { return KS ? (row & 3) << 1 : kRow == 8 ? row & 7 : (row >> 1) & 3; }
+  // place p holds row p / kRow and piece (p % kRow) ^ permute(row).  64 banks serve 256 bytes a cycle: k-fast reads take one
+  // piece of 16 rows together, k-slow reads 64 bytes of 4 consecutive k.
+  static __device__ __forceinline__ int permute(int row) {
+    if constexpr (KS) return kRow == 8 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+    else return kRow == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+  }
 
   // Registers: a thread's pieces of the tile at row r0 (of r_end) and k0 (of k_end); zeros past both ends.
   static __device__ __forceinline__ void load(Raw8<T> (&raw)[kEach], const E* base, long long ld, int r0, int r_end, int k0, int k_end) {
@@ -217,22 +267,40 @@ struct Tile {
   }
 
   // Straight into LDS (16-bit types, rows on 16-byte boundaries): a wavefront writes 1 KiB of consecutive places.  A piece
-  // that is not there gets an address past the buffer's end, for which the hardware's bounds check delivers zeros.
-  static __device__ __forceinline__ void load_direct(char* lds, const E* base, long long ld, int r0, int r_end, int k0, int k_end) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const E* corner = base + (KS ? (long long)k0 * ld + r0 : (long long)r0 * ld + k0);
-    // bytes from the corner that any piece inside the operand can reach
-    const long long rows = KS ? k_end - k0 : r_end - r0, last = KS ? r_end - r0 : k_end - k0;
-    const long long span = ((rows - 1) * ld + last) * 2;
-    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(corner), 0, (int)(span < 0x7ffffff0ll ? span : 0x7ffffff0ll), 0x00020000);
+  // that is not there gets an address past the buffer's end, for which the hardware's bounds check delivers zeros.  One tile
+  // after the other, each BK further along k.  Past the end the pieces are zeros.
+  struct Source {
+    const E* corner;
+    long long span, step;  // bytes left from the corner; bytes a tile further
+    int left;              // k left
+    int offset[kEach], k[kEach];
+    __device__ __forceinline__ void init(const E* base, long long ld, int r0, int r_end, int k0, int k_end) {
+      corner = base + (KS ? (long long)k0 * ld + r0 : (long long)r0 * ld + k0);
+      const long long rows = KS ? k_end - k0 : r_end - r0, last = KS ? r_end - r0 : k_end - k0;
+      span = ((rows - 1) * ld + last) * 2;
+      step = (KS ? BK * ld : BK) * 2;
+      left = k_end - k0;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int p = j * THREADS + threadIdx.x, row = p / kRow, piece = (p % kRow) ^ permute(row);
-      const bool in = KS ? k0 + row < k_end && r0 + 8 * piece < r_end : r0 + row < r_end && k0 + 8 * piece < k_end;
-      const int offset = in ? (row * (int)ld + 8 * piece) * 2 : 0x7ffffff0;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + (j * THREADS + wave * 64) * 16), 16, offset, 0, 0, 0);
+      for (int j = 0; j < kEach; ++j) {
+        const int p = j * THREADS + threadIdx.x, row = p / kRow, piece = (p % kRow) ^ permute(row);
+        k[j] = KS ? row : 8 * piece;
+        offset[j] = (KS ? r0 + 8 * piece < r_end : r0 + row < r_end) ? (row * (int)ld + 8 * piece) * 2 : 0x7ffffff0;
+      }
     }
-  }
+    __device__ __forceinline__ void next(char* lds) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass has no type for the buffer descriptor and would drop the kernel's launch stub
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(corner), 0, (int)(span < 0 ? 0 : span < 0x7ffffff0ll ? span : 0x7ffffff0ll), 0x00020000);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + (j * THREADS + wave * 64) * 16), 16,
+                                                 k[j] < left ? offset[j] : 0x7ffffff0, 0, 0, 0);
+      corner = left > BK ? corner + step / 2 : corner;  // past the end nothing is read: the address stays inside
+      span -= step;
+      left -= BK;
+#endif
+    }
+  };
 
   // The eight k of rows r .. r+31 (one a lane, twice) that step s of 16 k takes: lanes 32.. have the second eight.
   static __device__ __forceinline__ u4 frag(const char* lds, int r, int s, int lane) {
@@ -264,50 +332,174 @@ struct GemmArgs {
   const void *a, *b;
   long long a_ld, b_ld;
   int M, N, K;
-  int tiles_m, tiles_n, splits, k_each;  // k_each: multiple of BK, the k that one of the splits takes
-  float* partial;                        // splits > 1: [splits][M][N]
+  // `whole` tiles of the result are done by one block each; the others are cut along k into `splits` pieces of k_each (a
+  // multiple of BK), whose float32 results go to partial: [other tile][split][BM][BN]
+  int tiles_m, tiles_n, whole, splits, k_each;
+  float* partial;
   Epilogue e;
 };
 
 // A float32 result that is NaN may owe it to the split of an infinite or overflowing operand: it is computed again in
 // float32.  Nothing of a finite product comes here.
 template <bool A_KS, bool B_KS>
-__device__ __attribute__((noinline)) float product_again(const float* a, const float* b, long long a_ld, long long b_ld, long long m, int n, int k0, int k1) {
+__device__ __forceinline__ float product_again(const float* a, const float* b, long long a_ld, long long b_ld, long long m, int n, int k0, int k1) {
   float s = 0.f;
   for (int k = k0; k < k1; ++k)
     s = fmaf(A_KS ? a[(long long)k * a_ld + m] : a[m * a_ld + k], B_KS ? b[(long long)k * b_ld + n] : b[(long long)n * b_ld + k], s);
   return s;
 }
 
-// Blocks are dealt to the 8 XCDs in turn; consecutive work of one XCD shares operands in its L2, so tiles are numbered
-// XCD by XCD, and inside that in columns of 8 tile rows.
-__device__ __forceinline__ void tile_of(const GemmArgs& g, int& tm, int& tn, int& split) {
-  const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits, id = blockIdx.x;
-  const int xcd = id & 7, each = total >> 3, rest = total & 7;
-  const int w = xcd * each + min(xcd, rest) + (id >> 3);
-  split = w / tiles;
-  const int t = w - split * tiles, band = 8 * g.tiles_n, band_id = t / band, in = t - band_id * band;
-  const int rows = min(8, g.tiles_m - 8 * band_id);
+// What a wavefront's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// All but this wavefront's last N loads into LDS have landed, its LDS reads are done, and every wavefront is here.
+template <int N>
+__device__ __forceinline__ void landed() {
+  static_assert(N < 64, "");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (0 << 8));  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The i-th tile of the result: columns of 8 tile rows, so that tiles in work at the same time share operands.
+__device__ __forceinline__ void place_of(const GemmArgs& g, int i, int& tm, int& tn) {
+  const int band = 8 * g.tiles_n, band_id = i / band, in = i - band_id * band, rows = min(8, g.tiles_m - 8 * band_id);
   tm = 8 * band_id + in % rows;
   tn = in / rows;
 }
 
-// WM x WN of the result per wavefront in 32 x 32 blocks; two LDS buffers, the next tile on its way while one is used.
-template <class T, bool A_KS, bool B_KS, int BM, int BN, int BK, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm(GemmArgs g) {
+// The i-th of n pieces of work for this block.  Blocks are dealt to the 8 XCDs in turn; each XCD gets a consecutive run, as
+// it has an L2 of its own.
+__device__ __forceinline__ int dealt(int id, int n) {
+  const int xcd = id & 7, each = n >> 3, rest = n & 7;
+  return xcd * each + min(xcd, rest) + (id >> 3);
+}
+
+struct Work {
+  int tm, tn, k0, k1;
+  float* partial;  // null: the tile is whole
+};
+template <int BM, int BN>
+__device__ __forceinline__ Work work_of(const GemmArgs& g) {
+  Work w;
+  const int id = blockIdx.x;
+  if (id < g.whole) {
+    place_of(g, dealt(id, g.whole), w.tm, w.tn);
+    w.k0 = 0;
+    w.k1 = g.K;
+    w.partial = nullptr;
+  } else {
+    // the splits of a tile next to one another: they share nothing, but neighbours of the same split do
+    const int others = g.tiles_m * g.tiles_n - g.whole, i = dealt(id - g.whole, others * g.splits), split = i / others, tile = i - split * others;
+    place_of(g, g.whole + tile, w.tm, w.tn);
+    w.k0 = split * g.k_each;
+    w.k1 = min(g.K, w.k0 + g.k_each);
+    w.partial = g.partial + ((long long)tile * g.splits + split) * (BM * BN);
+  }
+  return w;
+}
+
+// A wavefront's 32 IM x 32 IN block of the result, through LDS into rows: eight consecutive n a lane, 32 rows by (up to) 64
+// columns at a time.  Pieces of four are permuted by the row, as lanes write one column of 32 rows.  lds: kWayOut bytes of
+// this wavefront, not in use for anything else.
+template <int IN>
+constexpr int kWayOut = 32 * 32 * (IN < 2 ? IN : 2) * 4;
+template <class T, bool A_KS, bool B_KS, int BN, int IM, int IN>
+__device__ __forceinline__ void write_result(const GemmArgs& g, f16v (&acc)[IM][IN], char* lds, int m0, int n0, const Work& w, int wm, int wn) {
+  // w.partial: [BM][BN], of which this wavefront's block begins at wm, wn
+  constexpr int JN = IN < 2 ? IN : 2, WN = 32 * JN, kQuads = WN / 4, kPerRow = WN / 8, kRows = 64 / kPerRow;
+  static_assert(IN % JN == 0, "");
+  using E = typename T::elem;
+  const E *a = static_cast<const E*>(g.a), *b = static_cast<const E*>(g.b);
+  const int lane = threadIdx.x & 63;
+  float* mine = reinterpret_cast<float*>(lds);
+  const int quad_mask = kQuads < 16 ? kQuads - 1 : 15;
+  DropArgs drop = g.e.drop;
+  if (drop.drop) load_offset(drop);
+#pragma unroll
+  for (int i = 0; i < IM; ++i) {
+#pragma unroll
+    for (int j0 = 0; j0 < IN; j0 += JN) {
+      wave_fence();
+#pragma unroll
+      for (int j = 0; j < JN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = lane & 31, quad = (8 * j + 2 * q + (lane >> 5)) ^ (row & quad_mask);
+          const f16v& r = acc[i][j0 + j];
+          *reinterpret_cast<f4*>(mine + row * WN + 4 * quad) = f4{r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]};
+        }
+      wave_fence();
+      const int c = lane % kPerRow, n = n0 + 32 * j0 + 8 * c, left = g.N - n;
+      if (left <= 0) continue;
+      constexpr int G = 2;  // rows a lane has in hand at a time: what registers the accumulators leave
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += G * kRows) {
+        float v[G][8];
+        long long m[G];
+        auto place = [&](int r, int half) {  // of four values of this lane
+          const int row = r0 + r * kRows + lane / kPerRow;
+          return mine + row * WN + 4 * ((2 * c + half) ^ (row & quad_mask));
+        };
+        auto take = [&] {
+#pragma unroll
+          for (int r = 0; r < G; ++r) {
+            const f4 lo = *reinterpret_cast<const f4*>(place(r, 0)), hi = *reinterpret_cast<const f4*>(place(r, 1));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              v[r][x] = lo[x];
+              v[r][4 + x] = hi[x];
+            }
+            m[r] = m0 + 32 * i + r0 + r * kRows + lane / kPerRow;
+          }
+        };
+        take();
+        if constexpr (kPlanes<T> == 3) {
+          bool bad = false;
+#pragma unroll
+          for (int r = 0; r < G; ++r)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) bad |= v[r][x] != v[r][x];
+          if (__any(bad)) {
+#pragma unroll 1
+            for (int t = 0; t < G * 8; ++t) {
+              const int r = t >> 3, x = t & 7;
+              const long long row = m0 + 32 * i + r0 + r * kRows + lane / kPerRow;
+              float* p = place(r, x >> 2) + (x & 3);
+              if (*p != *p && x < left && row < g.M) *p = product_again<A_KS, B_KS>(a, b, g.a_ld, g.b_ld, row, n + x, w.k0, w.k1);
+            }
+            take();
+          }
+        }
+        if (w.partial) {
+#pragma unroll
+          for (int r = 0; r < G; ++r) store8<Fp32>(w.partial + (wm + m[r] - m0) * BN + wn + n - n0, v[r]);
+        } else {
+          finish<T, G>(g.e, drop, m, g.M, n, left, v);
+        }
+      }
+    }
+  }
+}
+
+// Any alignment and type: tiles come through registers, where float32 is split.  WM x WN of the result per wavefront.
+// The next tile is on its way while one is multiplied, and other blocks of the CU multiply while this one splits and stores.
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int BK, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 1) void k_layer_gemm(GemmArgs g) {
   constexpr int kThreads = (BM / WM) * (BN / WN) * 64, IM = WM / 32, IN = WN / 32;
   using TA = Tile<T, A_KS, BM, BK, kThreads>;
   using TB = Tile<T, B_KS, BN, BK, kThreads>;
   using E = typename T::elem;
-  constexpr int kStage = TA::kBytes + TB::kBytes, kOut = (kThreads / 64) * 32 * WN * 4;
-  // two objects, so that the compiler sees that a tile on its way does not touch the one being read
-  __shared__ __attribute__((aligned(16))) char buf0[kStage > kOut ? kStage : kOut];
-  __shared__ __attribute__((aligned(16))) char buf1[kStage];
+  constexpr int kStage = TA::kBytes + TB::kBytes, kOut = (kThreads / 64) * kWayOut<IN>;
+  __shared__ __attribute__((aligned(16))) char buf[kStage > kOut ? kStage : kOut];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-  int tm, tn, split;
-  tile_of(g, tm, tn, split);
-  const int m0 = tm * BM, n0 = tn * BN, k0 = split * g.k_each, k1 = min(g.K, k0 + g.k_each);
+  const Work w = work_of<BM, BN>(g);
+  const int m0 = w.tm * BM, n0 = w.tn * BN, k0 = w.k0, k1 = w.k1;
   const E *a = static_cast<const E*>(g.a), *b = static_cast<const E*>(g.b);
 
   f16v acc[IM][IN];
@@ -318,21 +510,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm(GemmA
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  Raw8<T> ra[DIRECT ? 1 : TA::kEach], rb[DIRECT ? 1 : TB::kEach];
-  auto fetch = [&](char* buf, int k) {
-    if constexpr (DIRECT) {
-      TA::load_direct(buf, a, g.a_ld, m0, g.M, k, k1);
-      TB::load_direct(buf + TA::kBytes, b, g.b_ld, n0, g.N, k, k1);
-    } else {
-      TA::load(ra, a, g.a_ld, m0, g.M, k, k1);
-      TB::load(rb, b, g.b_ld, n0, g.N, k, k1);
-    }
+  Raw8<T> ra[TA::kEach], rb[TB::kEach];
+  auto fetch = [&](int k) {
+    TA::load(ra, a, g.a_ld, m0, g.M, k, k1);
+    TB::load(rb, b, g.b_ld, n0, g.N, k, k1);
   };
   auto put = [&](char* buf) {
-    if constexpr (!DIRECT) {
-      TA::store(ra, buf);
-      TB::store(rb, buf + TA::kBytes);
-    }
+    TA::store(ra, buf);
+    TB::store(rb, buf + TA::kBytes);
   };
   auto multiply = [&](const char* buf) {
 #pragma unroll
@@ -356,63 +541,90 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm(GemmA
             for (int j = 0; j < IN; ++j) acc[i][j] = mfma<T>(fb[pb][j], fa[pa][i], acc[i][j]);
     }
   };
-  auto step = [&](char* now, char* next, int k) {
-    const bool more = k + BK < k1;
-    if (more) fetch(next, k + BK);
-    multiply(now);
-    if (more) put(next);
+  fetch(k0);
+  for (int k = k0; k < k1; k += BK) {
+    put(buf);
     __syncthreads();
-  };
-  fetch(buf0, k0);
-  put(buf0);
-  __syncthreads();
-  for (int k = k0; k < k1; k += 2 * BK) {
-    step(buf0, buf1, k);
-    if (k + BK < k1) step(buf1, buf0, k + BK);
+    if (k + BK < k1) fetch(k + BK);
+    multiply(buf);
+    __syncthreads();
   }
+  write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, buf + wave * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
+}
 
-  // Through LDS into rows: eight consecutive n a lane, 32 rows of this wavefront at a time.  Pieces of four are permuted
-  // by the row, as lanes write one column of 32 rows.
-  constexpr int kQuads = WN / 4, kPerRow = WN / 8, kRows = 64 / kPerRow;
-  float* mine = reinterpret_cast<float*>(buf0) + wave * 32 * WN;
-  const int quad_mask = kQuads < 16 ? kQuads - 1 : 15;
-  DropArgs drop = g.e.drop;
-  if (drop.drop) load_offset(drop);
+// Operands of 16-bit types on 16-byte boundaries: tiles of 32 k go straight from memory into a ring of four LDS buffers, with one
+// barrier a step: it tells that a tile has landed for every wavefront (each waits for its own part) and that nobody reads
+// the oldest one any more, whose buffer is then filled again.
+// While step t is multiplied, tiles t+2 and t+3 are on their way and t+1 is there, so that its first fragments are read before
+// the barrier that ends the step.
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm_ring(GemmArgs g) {
+  constexpr int kThreads = (BM / WM) * (BN / WN) * 64, IM = WM / 32, IN = WN / 32, BK = 32;
+  using TA = Tile<T, A_KS, BM, BK, kThreads>;
+  using TB = Tile<T, B_KS, BN, BK, kThreads>;
+  using E = typename T::elem;
+  constexpr int kStage = TA::kBytes + TB::kBytes, kLoads = TA::kEach + TB::kEach, kHalf = kThreads / 128;
+  static_assert(kHalf * kWayOut<IN> <= kStage, "half of the wavefronts have their way out in the first buffer, half in the second");
+  // objects of their own, so that the compiler sees that a tile on its way does not touch the ones being read
+  __shared__ __attribute__((aligned(16))) char buf0[kStage], buf1[kStage], buf2[kStage], buf3[kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
+  const Work w = work_of<BM, BN>(g);
+  const int m0 = w.tm * BM, n0 = w.tn * BN, k0 = w.k0, k1 = w.k1;
+  typename TA::Source sa;
+  typename TB::Source sb;
+  sa.init(static_cast<const E*>(g.a), g.a_ld, m0, g.M, k0, k1);
+  sb.init(static_cast<const E*>(g.b), g.b_ld, n0, g.N, k0, k1);
+
+  f16v acc[IM][IN];
 #pragma unroll
-  for (int i = 0; i < IM; ++i) {
-    __syncthreads();
+  for (int i = 0; i < IM; ++i)
 #pragma unroll
     for (int j = 0; j < IN; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int row = lane & 31, quad = (8 * j + 2 * q + (lane >> 5)) ^ (row & quad_mask);
-        *reinterpret_cast<f4*>(mine + row * WN + 4 * quad) = f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-      }
-    __syncthreads();
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  auto fetch = [&](char* buf) {
+    sa.next(buf);
+    sb.next(buf + TA::kBytes);
+  };
+  u4 fa[2][IM], fb[2][IN];
+  auto read = [&](int set, const char* buf, int s) {
 #pragma unroll
-    for (int r = 0; r < 32 / kRows; ++r) {
-      const int row = r * kRows + lane / kPerRow, c = lane % kPerRow;
-      const f4 lo = *reinterpret_cast<const f4*>(mine + row * WN + 4 * ((2 * c) ^ (row & quad_mask)));
-      const f4 hi = *reinterpret_cast<const f4*>(mine + row * WN + 4 * ((2 * c + 1) ^ (row & quad_mask)));
-      float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      const long long m = m0 + wm + 32 * i + row;
-      const int n = n0 + wn + 8 * c, left = g.N - n;
-      if (m < g.M && left > 0) {
-        if constexpr (kPlanes<T> == 3) {
+    for (int j = 0; j < IN; ++j) fb[set][j] = TB::frag(buf + TA::kBytes, wn + 32 * j, s, lane);
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            if (v[x] != v[x] && x < left) v[x] = product_again<A_KS, B_KS>(a, b, g.a_ld, g.b_ld, m, n + x, k0, k1);
-        }
-        if (g.splits > 1) {
-          float* p = g.partial + ((long long)split * g.M + m) * g.N + n;
-          if (left >= 8) store8<Fp32>(p, v);
-          else store_some<Fp32>(p, left, v);
-        } else {
-          finish8<T>(g.e, drop, m, n, left, v);
-        }
-      }
-    }
+    for (int i = 0; i < IM; ++i) fa[set][i] = TA::frag(buf, wm + 32 * i, s, lane);
+  };
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+      for (int j = 0; j < IN; ++j) acc[i][j] = mfma<T>(fb[set][j], fa[set][i], acc[i][j]);
+  };
+  auto step = [&](const char* now, const char* next, char* free) {
+    fetch(free);
+    read(1, now, 1);
+    multiply(0);
+    read(0, next, 0);
+    multiply(1);
+    landed<kLoads>();
+  };
+  fetch(buf0);
+  fetch(buf1);
+  fetch(buf2);
+  landed<kLoads>();
+  read(0, buf0, 0);
+  for (int left = (k1 - k0 + BK - 1) / BK;;) {
+    step(buf0, buf1, buf3);
+    if (--left == 0) break;
+    step(buf1, buf2, buf0);
+    if (--left == 0) break;
+    step(buf2, buf3, buf1);
+    if (--left == 0) break;
+    step(buf3, buf0, buf2);
+    if (--left == 0) break;
   }
+  __syncthreads();  // also waits for the tiles past the end, which are still on their way
+  write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, (wave < kHalf ? buf0 : buf1) + (wave % kHalf) * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
 }
 
 }  // namespace

@@ -8,8 +8,9 @@ namespace {
 template <class T, int PRODUCT, int BM, int BN, int BK, int WM, int WN, bool DIRECT>
 int launch_gemm(const GemmArgs& g, hipStream_t st) {
   constexpr bool kASlow = PRODUCT == kKernelGrad, kBSlow = PRODUCT != kInputGrad;
-  k_layer_gemm<T, kASlow, kBSlow, BM, BN, BK, WM, WN, DIRECT>
-      <<<(unsigned)(g.tiles_m * g.tiles_n * g.splits), (BM / WM) * (BN / WN) * 64, 0, st>>>(g);
+  const unsigned grid = (unsigned)(g.whole + (g.tiles_m * g.tiles_n - g.whole) * g.splits), block = (BM / WM) * (BN / WN) * 64;
+  if constexpr (DIRECT) k_layer_gemm_ring<T, kASlow, kBSlow, BM, BN, WM, WN><<<grid, block, 0, st>>>(g);
+  else k_layer_gemm<T, kASlow, kBSlow, BM, BN, BK, WM, WN><<<grid, block, 0, st>>>(g);
   return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
 }
 
@@ -17,8 +18,8 @@ template <class T, int PRODUCT, bool DIRECT>
 int launch_block(int block, const GemmArgs& g, hipStream_t st) {
   constexpr int BK = kPlanes<T> == 3 ? 32 : 64;
   switch (block) {
-    case kBlock32x128:
-      if constexpr (PRODUCT != kKernelGrad) return launch_gemm<T, PRODUCT, 32, 128, 64, 32, 32, DIRECT>(g, st);
+    case kBlock32:
+      if constexpr (PRODUCT != kKernelGrad) return launch_gemm<T, PRODUCT, 32, DIRECT ? 64 : 128, 64, 32, 32, DIRECT>(g, st);
       break;
     case kBlock64x64: return launch_gemm<T, PRODUCT, 64, 64, BK, 32, 32, DIRECT>(g, st);
     case kBlock128x128: return launch_gemm<T, PRODUCT, 128, 128, BK, 64, 64, DIRECT>(g, st);

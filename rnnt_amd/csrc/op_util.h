@@ -9,6 +9,9 @@
 
 namespace {
 
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -39,6 +42,14 @@ __device__ __forceinline__ uint32_t float_to_bf16_bits(float v) {
   uint16_t b;
   __builtin_memcpy(&b, &f, 2);
   return b;
+}
+
+// two at a time: one instruction
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), bf2));
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), hf2));
 }
 
 template <class T>
@@ -96,8 +107,8 @@ __device__ __forceinline__ void store8(typename T::elem* p, const float (&v)[8])
     u4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (T::code == RNNT_MI355X_BF16) w[i] = float_to_bf16_bits(v[2 * i]) | (float_to_bf16_bits(v[2 * i + 1]) << 16);
-      else w[i] = float_to_half_bits(v[2 * i]) | (float_to_half_bits(v[2 * i + 1]) << 16);
+      if constexpr (T::code == RNNT_MI355X_BF16) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      else w[i] = pack_half(v[2 * i], v[2 * i + 1]);
     }
     d[0] = w;
   }
@@ -144,6 +155,10 @@ __device__ __forceinline__ void load_offset(DropArgs& a) {
   }
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction for the truth table of a ^ b ^ c
+}
+
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011): ten rounds of two
 // 32x32-bit products over a counter of four words, of which every value gives 128 independent bits.  Eight columns of a
 // row share a counter and take 16 bits each: with 32 bits the generator (20 wide products, ~60 cycles an element-quad on
@@ -152,9 +167,9 @@ __device__ __forceinline__ u4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(q >> 32), c1, k0);
     c1 = (uint32_t)q;
-    c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(p >> 32), c3, k1);
     c3 = (uint32_t)p;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
