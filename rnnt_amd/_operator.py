@@ -18,7 +18,7 @@ def stream(device) -> int:
 
 def on_device(device):
     """Makes `device` current for a launch where it is not already."""
-    return _ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _ALREADY if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 class _Already:

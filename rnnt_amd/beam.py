@@ -8,6 +8,7 @@ of beams in one or two launches straight from the joint's logits (log-softmax in
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -90,31 +91,34 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
     batch_dim + 1 are (B, K) -- [layers, B, K, hidden] has batch_dim 1.  Returns a list with W in the place of K and row
     parent[b, w] of utterance b at [b, w]; zeros where parent is -1 (any value outside [0, K)).  out: tensors to write to
     instead of new ones, dense, of the results' shapes and types, sharing no memory with states or one another."""
-    if parent.dtype != torch.int32 or parent.dim() != 2:
+    if not isinstance(parent, torch.Tensor) or parent.dtype != torch.int32 or parent.dim() != 2:
         raise ValueError("beam_reorder: parent must be int32 [B, W]")
     states = list(states)
-    dev = need_gpu("beam_reorder", parent=parent, **{f"states[{i}]": s for i, s in enumerate(states)})
+    dev = need_gpu("beam_reorder", parent=parent)
+    for i, s in enumerate(states):
+        if not isinstance(s, torch.Tensor) or s.device != dev:
+            need_gpu("beam_reorder", parent=parent, **{f"states[{i}]": s})
     B, W = parent.shape
     d = int(batch_dim)
     if d < 0:
         raise ValueError("beam_reorder: batch_dim counts from the first dimension")
-    K = None
+    K = -1
+    new, todo, keep = [], [], [parent if parent.is_contiguous() else parent.contiguous()]
     for i, s in enumerate(states):
-        if s.dim() < d + 2 or s.shape[d] != B:
-            raise ValueError(f"beam_reorder: states[{i}] has shape {tuple(s.shape)}, expected B={B} at dimension {d} and the beams next")
-        if K is None:
-            K = s.shape[d + 1]
-        elif s.shape[d + 1] != K:
+        shape = s.shape
+        if len(shape) < d + 2 or shape[d] != B:
+            raise ValueError(f"beam_reorder: states[{i}] has shape {tuple(shape)}, expected B={B} at dimension {d} and the beams next")
+        if K < 0:
+            K = shape[d + 1]
+        elif shape[d + 1] != K:
             raise ValueError("beam_reorder: the states differ in their number of beams")
-    if not states:
-        return []
-    shapes = [s.shape[:d + 1] + (W,) + s.shape[d + 2:] for s in states]
+        new.append((*shape[:d + 1], W, *shape[d + 2:]))
     if out is None:
-        out = [torch.empty(shape, dtype=s.dtype, device=dev) for s, shape in zip(states, shapes)]
+        out = [torch.empty(shape, dtype=s.dtype, device=dev) for s, shape in zip(states, new)]
     else:
         out = list(out)
         need_gpu("beam_reorder", parent=parent, **{f"out[{i}]": o for i, o in enumerate(out)})
-        if len(out) != len(states) or any(o.shape != sh or o.dtype != s.dtype or not o.is_contiguous() for o, s, sh in zip(out, states, shapes)):
+        if len(out) != len(states) or any(o.shape != sh or o.dtype != s.dtype or not o.is_contiguous() for o, s, sh in zip(out, states, new)):
             raise ValueError("beam_reorder: out must be dense tensors of the results' shapes and types")
         spans = [(*_bytes_of(t), i < len(out)) for i, t in enumerate([*out, *states, parent]) if t.numel()]
         for i, (a0, a1, written) in enumerate(spans):
@@ -124,23 +128,19 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
         for o in out:
             o.zero_()
         return out
-    parent = parent.contiguous()
-    keep, todo = [], []
     for s, o in zip(states, out):
         if o.numel() == 0:
             continue
         # [outer, B, K, row]: the row has to be dense, the three leading dimensions need one stride each
-        tail_dense = s.shape[d + 2:].numel() <= 1 or s[(0,) * (d + 2)].is_contiguous()
-        if not tail_dense or d > 1:
+        if not s.is_contiguous() and (d > 1 or not s[(0,) * (d + 2)].is_contiguous()):
             s = s.contiguous()
-        keep.append(s)
-        e = s.element_size()
-        outer = s.shape[:d].numel()
-        todo.append(_lib.ReorderTensor(s.data_ptr(), o.data_ptr(), outer, s.stride(0) * e if d == 1 else s.shape[d:].numel() * e,
-                                       s.stride(d) * e, s.stride(d + 1) * e, s.shape[d + 2:].numel() * e))
+            keep.append(s)
+        e, strides = s.element_size(), s.stride()
+        row, outer = math.prod(s.shape[d + 2:]), math.prod(s.shape[:d])
+        todo.append(_lib.ReorderTensor(s.data_ptr(), o.data_ptr(), outer, strides[d - 1] * e if d else 0, strides[d] * e, strides[d + 1] * e, row * e))
     with on_device(dev):
         for i in range(0, len(todo), _lib.REORDER_MAX):
             part = todo[i:i + _lib.REORDER_MAX]
-            rc = _lib.lib().rnnt_mi355x_beam_reorder((_lib.ReorderTensor * len(part))(*part), len(part), parent.data_ptr(), B, K, W, stream(dev))
+            rc = _lib.lib().rnnt_mi355x_beam_reorder((_lib.ReorderTensor * len(part))(*part), len(part), keep[0].data_ptr(), B, K, W, stream(dev))
             check(rc, "rnnt_mi355x_beam_reorder")
     return out

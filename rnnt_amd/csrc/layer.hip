@@ -83,8 +83,7 @@ __global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a) {
       if (a.drop.drop) drop8(a.drop, (uint32_t)m, (uint32_t)n0 >> 3, v);
       if (a.dz) {
         typename T::elem* q = static_cast<typename T::elem*>(a.dz) + m * a.dz_ld + n0;
-        if (left >= 8) store8<T>(q, v);
-        else store_some<T>(q, left, v);
+        store8<T>(q, v);  // whole pieces: what lies behind the last column is zero
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += v[i];
@@ -103,23 +102,43 @@ __global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a) {
   }
 }
 
-// db: the row blocks' sums, 64 columns and 16 blocks at a time; the order is fixed.
+// db: the row blocks' sums, 32 columns and 32 blocks at a time; the order is fixed.
 template <class T>
 __global__ __launch_bounds__(1024) void k_layer_db(const float* partial, int blocks, int N, typename T::elem* db) {
-  __shared__ float sums[16][64];
-  const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
   float s = 0.f;
   if (n < N) {
 #pragma unroll 8
-    for (int i = r; i < blocks; i += 16) s += partial[(long long)i * N + n];
+    for (int i = r; i < blocks; i += 32) s += partial[(long long)i * N + n];
   }
   sums[r][c] = s;
   __syncthreads();
   if (r == 0 && n < N) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += sums[i][c];
+    for (int i = 1; i < 32; ++i) s += sums[i][c];
     db[n] = from_float<T>(s);
   }
+}
+
+// ---- rows that do not lie on 16-byte boundaries --------------------------------------------------------------------------
+// A 16-bit matrix copied to rows of whole 16-byte pieces, zeros behind the last column: with it the products take the
+// ring kernel.
+struct PackArgs {
+  const uint16_t* src;
+  uint16_t* dst;
+  long long src_ld, dst_ld, rows;
+  int cols;
+};
+__global__ __launch_bounds__(256) void k_layer_pack(PackArgs a, PackArgs b, unsigned a_blocks) {
+  const PackArgs p = blockIdx.x < a_blocks ? a : b;
+  const long long block = blockIdx.x < a_blocks ? blockIdx.x : blockIdx.x - a_blocks;
+  const int pieces = (p.cols + 7) / 8;
+  const long long id = block * 256 + threadIdx.x, row = id / pieces;
+  if (row >= p.rows) return;
+  const int c = (int)(id - row * pieces) * 8;
+  const Raw8<Bf16> r = load_group<Bf16>(p.src + row * p.src_ld + c, p.cols - c);
+  *reinterpret_cast<u4*>(p.dst + row * p.dst_ld + c) = r.q[0];
 }
 
 // ---- joining the splits of a product -------------------------------------------------------------------------------------
@@ -158,6 +177,106 @@ __global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn) 
   finish<T, 1>(g.e, drop, {m}, g.M, n, left, v);
 }
 
+// ---- a decoder's few rows ------------------------------------------------------------------------------------------------
+constexpr int kRowsMost = 8, kRowsSlices = 16, kRowsChunk = 1024;
+template <class T>
+constexpr int kRowsVec = T::code == RNNT_MI355X_FP32 ? 1 : 2;  // columns a lane: a wavefront reads 256 bytes of a row of W
+
+// x W for at most 8 rows: bound by the read of W, or by a launch and a few memory latencies for a small one, where the
+// matrix cores' tiles of 32 rows would be mostly empty.  A block has 64 or 128 columns; its 16 wavefronts share k, each reads
+// its rows of W straight into registers, 16 at a time, and takes x from LDS.  The sums of the wavefronts meet in LDS.
+template <class T, int MR>
+__global__ __launch_bounds__(64 * kRowsSlices) void k_layer_rows(GemmArgs g) {
+  using E = typename T::elem;
+  constexpr int VEC = kRowsVec<T>, BN = 64 * VEC, kRed = kRowsSlices * MR * BN, kX = MR * kRowsChunk;
+  __shared__ __attribute__((aligned(16))) float lds[kRed > kX ? kRed : kX];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % g.tiles_n, split = blockIdx.x / g.tiles_n;
+  const int n0 = tile * BN, n = n0 + VEC * lane, left = g.N - n;
+  const int k_begin = split * g.k_each, k_end = min(g.K, k_begin + g.k_each);
+  const E *x = static_cast<const E*>(g.a), *w = static_cast<const E*>(g.b);
+  float acc[MR][VEC];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) acc[m][v] = 0.f;
+
+  for (int k0 = k_begin; k0 < k_end; k0 += kRowsChunk) {
+    const int len = min(kRowsChunk, k_end - k0), each = ((len + kRowsSlices - 1) / kRowsSlices + 3) & ~3;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kX; i += 64 * kRowsSlices) {
+      const int m = i / kRowsChunk, k = i % kRowsChunk;
+      lds[i] = m < g.M && k < len ? to_float<T>(x[m * g.a_ld + k0 + k]) : 0.f;
+    }
+    __syncthreads();
+    const int first = wave * each, last = min(len, first + each);
+#pragma unroll 1
+    for (int k = first; k < last; k += 16) {
+      E q[16][VEC];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const E* p = w + (long long)(k0 + k + j) * g.b_ld + n;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) q[j][v] = 0;
+        if (k + j < last) {
+          if (left >= VEC) __builtin_memcpy(q[j], p, sizeof(q[j]));
+          else if (left > 0) q[j][0] = p[0];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+          const f4 a = *reinterpret_cast<const f4*>(lds + m * kRowsChunk + min(k + j, kRowsChunk - 4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+              // past the wavefront's last k the row of W was not read: nothing is added, also where x is no number
+              const float add = k + j + i < last ? a[i] : 0.f;
+              acc[m][v] = fmaf(add, to_float<T>(q[j + i][v]), acc[m][v]);
+            }
+        }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) lds[(wave * MR + m) * BN + VEC * lane + v] = acc[m][v];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MR * BN; i += 64 * kRowsSlices) {
+    float s = lds[i];
+#pragma unroll
+    for (int j = 1; j < kRowsSlices; ++j) s += lds[j * MR * BN + i];
+    lds[i] = s;  // this thread's own
+  }
+  __syncthreads();
+  constexpr int kGroups = BN / 8;
+  const int m = threadIdx.x / kGroups, c = 8 * (threadIdx.x % kGroups);
+  if (m >= MR || m >= g.M || n0 + c >= g.N) return;
+  float v[1][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[0][i] = lds[m * BN + c + i];
+  if (g.whole == 0) {
+    store8<Fp32>(g.partial + ((long long)tile * g.splits + split) * (kRowsMost * BN) + m * BN + c, v[0]);
+  } else {
+    DropArgs drop = g.e.drop;
+    if (drop.drop) load_offset(drop);
+    finish<T, 1>(g.e, drop, {m}, g.M, n0 + c, g.N - n0 - c, v);
+  }
+}
+
+template <class T>
+int launch_rows(const GemmArgs& g, hipStream_t st) {
+  const unsigned grid = (unsigned)(g.tiles_n * g.splits), block = 64 * kRowsSlices;
+  if (g.M == 1) k_layer_rows<T, 1><<<grid, block, 0, st>>>(g);
+  else if (g.M == 2) k_layer_rows<T, 2><<<grid, block, 0, st>>>(g);
+  else if (g.M <= 4) k_layer_rows<T, 4><<<grid, block, 0, st>>>(g);
+  else k_layer_rows<T, 8><<<grid, block, 0, st>>>(g);
+  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------
 struct Plan {
   int block, bm, bn, tiles_m, tiles_n, whole, splits, k_each;
@@ -176,6 +295,21 @@ Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
   p.bm = p.bn = 128;
   p.block = kBlock128x128;
   const int steps = ceil_div(K, 32);
+  if (product == kForward && M <= kRowsMost) {
+    // 256 blocks of 16 wavefronts if k allows pieces of 512 or more
+    p.block = kBlockRows;
+    p.bm = kRowsMost;
+    p.bn = dtype == RNNT_MI355X_FP32 ? 64 : 128;
+    p.tiles_m = 1;
+    p.tiles_n = ceil_div(N, p.bn);
+    p.splits = kCUs / p.tiles_n < K / 512 ? kCUs / p.tiles_n : K / 512;
+    if (p.splits < 2) p.splits = 1;
+    p.k_each = ceil_div(ceil_div(K, p.splits), 64) * 64;
+    p.splits = ceil_div(K, p.k_each);
+    p.whole = p.splits == 1 ? p.tiles_n : 0;
+    p.partial_bytes = p.whole ? 0 : (size_t)p.tiles_n * p.splits * p.bm * p.bn * sizeof(float);
+    return p;
+  }
   if (product != kKernelGrad && M <= 32) {
     p.block = kBlock32;
     p.bm = 32;
@@ -204,9 +338,9 @@ Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
   return p;
 }
 
-// 16-byte pieces that begin on 16-byte boundaries, in a tile whose byte offsets fit 31 bits.
-bool can_go_direct(const void* p, long long ld, int inner, int dtype) {
-  return dtype != RNNT_MI355X_FP32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && inner % 8 == 0 && ld < (1 << 21);
+// Rows of whole 16-byte pieces on 16-byte boundaries, in a tile whose byte offsets fit 31 bits.
+bool can_go_direct(const void* p, long long ld, int cols, int dtype) {
+  return dtype != RNNT_MI355X_FP32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld < (1 << 21);
 }
 
 size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -236,7 +370,7 @@ int run_product(int product, const Plan& p, const void* a, long long a_ld, const
   g.k_each = p.k_each;
   g.partial = partial;
   g.e = e;
-  const int rc = gemm_of<T>(product, p.block, p.direct, g, st);
+  const int rc = p.block == kBlockRows ? launch_rows<T>(g, st) : gemm_of<T>(product, p.block, p.direct, g, st);
   const int others = p.tiles_m * p.tiles_n - p.whole;
   if (rc != RNNT_MI355X_OK || others == 0) return rc;
   k_layer_join<T><<<(unsigned)others * (p.bm * p.bn / 256), 256, 0, st>>>(g, p.bm, p.bn);
@@ -276,40 +410,110 @@ int saved_by(const rnnt_mi355x_layer* l) {
 // row blocks of the dz pass: at most 1024 partial sums a column
 int dz_rows(long long M) { return M <= 65536 ? 64 : (int)((M + 1023) / 1024 + 7) / 8 * 8; }
 
-// dz's rows in the workspace.  Rows a multiple of 4 KiB apart put the same piece of all rows of a tile into the same few
-// memory channels: 32768 x 4096 x 1024 in bfloat16 ran 300 us with such rows and 257 us with rows 128 bytes longer.
-long long dz_stride(int out, int dtype) {
-  const long long e = dtype == RNNT_MI355X_FP32 ? 4 : 2;
-  return out * e % 4096 == 0 ? out + 128 / e : out;
+// Rows in the workspace: whole 16-byte pieces, and no multiple of 4 KiB apart, which puts the same piece of all rows of a
+// tile into the same few memory channels: 32768 x 4096 x 1024 in bfloat16 ran 300 us with such rows of x and 257 us with
+// rows 128 bytes longer.
+long long workspace_stride(int cols, int dtype) {
+  const long long e = dtype == RNNT_MI355X_FP32 ? 4 : 2, ld = ((long long)cols + 7) & ~7ll;
+  return ld * e % 4096 == 0 ? ld + 128 / e : ld;
+}
+
+// An operand as its product reads it: where it is, or copied to `at` of the workspace.
+struct Operand {
+  const void* p;
+  long long ld, rows;
+  int cols;
+  bool pack;
+  size_t at, bytes;
+};
+// Copying costs a read and a write of the operand; the product reads it at twice the speed or better.  6151 x 515 x 1030 in
+// float16, forward: 46 us from the rows as they are, 21 us copies included.  Operands that few rows use stay where they are.
+Operand operand(const void* p, long long ld, long long rows, int cols, int dtype, bool often) {
+  Operand o{p, ld, rows, cols, false, 0, 0};
+  if (dtype != RNNT_MI355X_FP32 && often && !can_go_direct(p, ld, cols, dtype) && cols < (1 << 20)) {
+    o.pack = true;
+    o.ld = workspace_stride(cols, dtype);
+    o.bytes = align_up((size_t)rows * o.ld * 2);
+  }
+  return o;
+}
+bool direct(const Operand& o, int dtype) { return o.pack || can_go_direct(o.p, o.ld, o.cols, dtype); }
+// The copies of a call, both in one launch; afterwards the operands are their copies.
+int pack(Operand& a, long long a_src_ld, Operand& b, long long b_src_ld, char* ws, hipStream_t st) {
+  PackArgs p[2];
+  unsigned blocks[2] = {0, 0};
+  Operand* o[2] = {&a, &b};
+  for (int i = 0; i < 2; ++i) {
+    p[i] = PackArgs{static_cast<const uint16_t*>(o[i]->p), reinterpret_cast<uint16_t*>(ws + o[i]->at), i ? b_src_ld : a_src_ld, o[i]->ld, o[i]->rows, o[i]->cols};
+    if (!o[i]->pack) continue;
+    const long long n = (o[i]->rows * ((o[i]->cols + 7) / 8) + 255) / 256;
+    if (n > 0x3fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
+    blocks[i] = (unsigned)n;
+    o[i]->p = ws + o[i]->at;
+  }
+  if (blocks[0] + blocks[1] == 0) return RNNT_MI355X_OK;
+  k_layer_pack<<<blocks[0] + blocks[1], 256, 0, st>>>(p[0], p[1], blocks[0]);
+  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+}
+
+constexpr int kOften = 512;  // rows that share the kernel
+
+struct ForwardPlan {
+  Operand x, kernel;
+  Plan y;
+  size_t partial_at, bytes;
+};
+ForwardPlan plan_forward(const rnnt_mi355x_layer* l) {
+  ForwardPlan f;
+  const bool often = l->rows >= kOften;
+  // x is read once for every 256 columns or fewer: worth a copy from a few blocks on
+  f.x = operand(l->x, l->x_stride, l->rows, l->in, l->dtype, often);
+  f.kernel = operand(l->kernel, l->kernel_stride, l->in, l->out, l->dtype, often);
+  f.kernel.at = f.x.at + f.x.bytes;
+  f.partial_at = f.kernel.at + f.kernel.bytes;
+  f.y = plan_product(kForward, l->dtype, (int)l->rows, l->out, l->in, direct(f.x, l->dtype) && direct(f.kernel, l->dtype));
+  f.bytes = f.partial_at + f.y.partial_bytes;
+  return f;
 }
 
 struct BackwardPlan {
   bool need_dz;  // else dz is dy
-  size_t dz_at, sums_at, partial_at, bytes;
+  Operand x, kernel, dz;
+  size_t sums_at, partial_at, bytes;
+  int dz_rows, dz_blocks;  // the dz pass: rows of a block, blocks
   Plan dx, dk;
 };
 BackwardPlan plan_backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride) {
   BackwardPlan b;
-  const int M = (int)l->rows;
-  const size_t e = l->dtype == RNNT_MI355X_FP32 ? 4 : 2;
-  b.need_dz = l->act != kLinear || l->drop16 != 0;
-  b.dz_at = 0;
-  b.sums_at = align_up(b.need_dz ? (size_t)M * dz_stride(l->out, l->dtype) * e : 0);
-  b.partial_at = b.sums_at + align_up((size_t)ceil_div(M, dz_rows(M)) * l->out * sizeof(float));
-  // dz lies in the workspace, on a 256-byte boundary
-  const bool dz_direct = b.need_dz ? l->dtype != RNNT_MI355X_FP32 && l->out % 8 == 0 && l->out < (1 << 21) : can_go_direct(dy, dy_stride, l->out, l->dtype);
-  b.dx = plan_product(kInputGrad, l->dtype, M, l->in, l->out, dz_direct && can_go_direct(l->kernel, l->kernel_stride, l->out, l->dtype));
-  b.dk = plan_product(kKernelGrad, l->dtype, l->in, l->out, M, dz_direct && can_go_direct(l->x, l->x_stride, l->in, l->dtype));
+  const int M = (int)l->rows, dtype = l->dtype;
+  const size_t e = dtype == RNNT_MI355X_FP32 ? 4 : 2;
+  const bool often = M >= kOften;
+  // the pass that makes dz also puts a dy whose rows lie badly on boundaries
+  b.need_dz = l->act != kLinear || l->drop16 != 0 || (often && dtype != RNNT_MI355X_FP32 && !can_go_direct(dy, dy_stride, l->out, dtype));
+  b.dz = Operand{dy, dy_stride, M, l->out, false, 0, 0};
+  if (b.need_dz) {
+    b.dz.ld = workspace_stride(l->out, dtype);
+    b.dz.pack = dtype != RNNT_MI355X_FP32 && b.dz.ld < (1 << 21);
+    b.dz.bytes = align_up((size_t)M * b.dz.ld * e);
+  }
+  b.x = operand(l->x, l->x_stride, M, l->in, dtype, often);
+  b.kernel = operand(l->kernel, l->kernel_stride, l->in, l->out, dtype, often);
+  b.x.at = b.dz.bytes;
+  b.kernel.at = b.x.at + b.x.bytes;
+  b.sums_at = b.kernel.at + b.kernel.bytes;
+  // 2048 blocks, in rows of 8
+  const long long across = ceil_div(l->out, kDzGroups * 8), rows = ((long long)M * across / 2048 + 7) / 8 * 8;
+  b.dz_rows = (int)(rows < 8 ? 8 : rows);
+  b.dz_blocks = ceil_div(M, b.dz_rows);
+  b.partial_at = b.sums_at + align_up((size_t)b.dz_blocks * l->out * sizeof(float));
+  b.dx = plan_product(kInputGrad, dtype, M, l->in, l->out, direct(b.dz, dtype) && direct(b.kernel, dtype));
+  b.dk = plan_product(kKernelGrad, dtype, l->in, l->out, M, direct(b.dz, dtype) && direct(b.x, dtype));
   b.bytes = b.partial_at + (b.dx.partial_bytes > b.dk.partial_bytes ? b.dx.partial_bytes : b.dk.partial_bytes);
   return b;
 }
-Plan plan_forward(const rnnt_mi355x_layer* l) {
-  return plan_product(kForward, l->dtype, (int)l->rows, l->out, l->in,
-                      can_go_direct(l->x, l->x_stride, l->in, l->dtype) && can_go_direct(l->kernel, l->kernel_stride, l->out, l->dtype));
-}
 
 template <class T>
-int forward(const rnnt_mi355x_layer* l, void* workspace, hipStream_t st) {
+int forward(const rnnt_mi355x_layer* l, ForwardPlan f, void* workspace, hipStream_t st) {
   Epilogue e = plain_output(l->y, l->out);
   e.bias = l->bias;
   e.residual = l->residual;
@@ -317,45 +521,48 @@ int forward(const rnnt_mi355x_layer* l, void* workspace, hipStream_t st) {
   e.aux = l->act == kLinear ? nullptr : l->aux;
   e.act = l->act;
   e.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
-  return run_product<T>(kForward, plan_forward(l), l->x, l->x_stride, l->kernel, l->kernel_stride, (int)l->rows, l->out, l->in, e,
-                        static_cast<float*>(workspace), st);
+  char* ws = static_cast<char*>(workspace);
+  const int rc = pack(f.x, l->x_stride, f.kernel, l->kernel_stride, ws, st);
+  if (rc != RNNT_MI355X_OK) return rc;
+  return run_product<T>(kForward, f.y, f.x.p, f.x.ld, f.kernel.p, f.kernel.ld, (int)l->rows, l->out, l->in, e, reinterpret_cast<float*>(ws + f.partial_at), st);
 }
 
 template <class T>
 int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, void* dx, void* dkernel, void* dbias, void* workspace, int from,
              hipStream_t st) {
-  const BackwardPlan b = plan_backward(l, dy, dy_stride);
+  BackwardPlan b = plan_backward(l, dy, dy_stride);
   const int M = (int)l->rows;
   char* ws = static_cast<char*>(workspace);
-  const void* dz = b.need_dz ? ws + b.dz_at : dy;
-  const long long dz_ld = b.need_dz ? dz_stride(l->out, l->dtype) : dy_stride;
+  if (b.need_dz) b.dz.p = ws + b.dz.at;
   float *sums = reinterpret_cast<float*>(ws + b.sums_at), *partial = reinterpret_cast<float*>(ws + b.partial_at);
-  const int blocks = ceil_div(M, dz_rows(M));
   if (b.need_dz || dbias) {
     DzArgs a;
     a.dy = dy;
     a.saved = from == kPreActivation ? l->aux : l->y;
-    a.dz = b.need_dz ? ws + b.dz_at : nullptr;
+    a.dz = b.need_dz ? ws + b.dz.at : nullptr;
     a.partial = dbias ? sums : nullptr;
     a.dy_ld = dy_stride;
-    a.dz_ld = dz_ld;
+    a.dz_ld = b.dz.ld;
     a.M = M;
     a.N = l->out;
-    a.rows = dz_rows(M);
+    a.rows = b.dz_rows;
     a.act = l->act;
     a.from = from;
     a.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
-    k_layer_dz<T><<<dim3((unsigned)ceil_div(l->out, kDzGroups * 8), (unsigned)blocks), kDzGroups * kDzLanes, 0, st>>>(a);
+    k_layer_dz<T><<<dim3((unsigned)ceil_div(l->out, kDzGroups * 8), (unsigned)b.dz_blocks), kDzGroups * kDzLanes, 0, st>>>(a);
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
   }
   if (dbias) {
-    k_layer_db<T><<<(unsigned)ceil_div(l->out, 64), 1024, 0, st>>>(sums, blocks, l->out, static_cast<typename T::elem*>(dbias));
+    k_layer_db<T><<<(unsigned)ceil_div(l->out, 32), 1024, 0, st>>>(sums, b.dz_blocks, l->out, static_cast<typename T::elem*>(dbias));
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
   }
-  int rc = RNNT_MI355X_OK;
-  if (dx) rc = run_product<T>(kInputGrad, b.dx, dz, dz_ld, l->kernel, l->kernel_stride, M, l->in, l->out, plain_output(dx, l->in), partial, st);
+  if (!dx) b.kernel.pack = false;
+  if (!dkernel) b.x.pack = false;
+  int rc = pack(b.x, l->x_stride, b.kernel, l->kernel_stride, ws, st);
+  if (rc == RNNT_MI355X_OK && dx)
+    rc = run_product<T>(kInputGrad, b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), partial, st);
   if (rc == RNNT_MI355X_OK && dkernel)
-    rc = run_product<T>(kKernelGrad, b.dk, l->x, l->x_stride, dz, dz_ld, l->in, l->out, M, plain_output(dkernel, l->out), partial, st);
+    rc = run_product<T>(kKernelGrad, b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), partial, st);
   return rc;
 }
 
@@ -366,7 +573,7 @@ extern "C" int rnnt_mi355x_layer_workspace_bytes(const rnnt_mi355x_layer* l, con
   const int rc = check_layer(l);
   if (rc != RNNT_MI355X_OK) return rc;
   if (backward_bytes && dy_stride < l->out) return RNNT_MI355X_INVALID_VALUE;
-  if (forward_bytes) *forward_bytes = plan_forward(l).partial_bytes;
+  if (forward_bytes) *forward_bytes = plan_forward(l).bytes;
   if (backward_bytes) *backward_bytes = plan_backward(l, dy, dy_stride).bytes;
   return RNNT_MI355X_OK;
 }
@@ -375,13 +582,14 @@ extern "C" int rnnt_mi355x_layer_forward(const rnnt_mi355x_layer* l, void* works
   const int rc = check_layer(l);
   if (rc != RNNT_MI355X_OK) return rc;
   if (!l->x || !l->kernel || !l->y || (l->residual && l->residual_stride < l->out)) return RNNT_MI355X_INVALID_VALUE;
-  if (!workspace && plan_forward(l).partial_bytes) return RNNT_MI355X_INVALID_VALUE;
+  const ForwardPlan f = plan_forward(l);
+  if (!workspace && f.bytes) return RNNT_MI355X_INVALID_VALUE;
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   switch (l->dtype) {
-    case RNNT_MI355X_FP32: return forward<Fp32>(l, workspace, st);
-    case RNNT_MI355X_BF16: return forward<Bf16>(l, workspace, st);
+    case RNNT_MI355X_FP32: return forward<Fp32>(l, f, workspace, st);
+    case RNNT_MI355X_BF16: return forward<Bf16>(l, f, workspace, st);
   }
-  return forward<Fp16>(l, workspace, st);
+  return forward<Fp16>(l, f, workspace, st);
 }
 
 extern "C" int rnnt_mi355x_layer_backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, void* dx, void* dkernel,

@@ -276,7 +276,8 @@ struct Tile {
     int offset[kEach], k[kEach];
     __device__ __forceinline__ void init(const E* base, long long ld, int r0, int r_end, int k0, int k_end) {
       corner = base + (KS ? (long long)k0 * ld + r0 : (long long)r0 * ld + k0);
-      const long long rows = KS ? k_end - k0 : r_end - r0, last = KS ? r_end - r0 : k_end - k0;
+      // rows are whole pieces long: a piece that begins inside is there to its end
+      const long long rows = KS ? k_end - k0 : r_end - r0, last = ((KS ? r_end - r0 : k_end - k0) + 7) & ~7;
       span = ((rows - 1) * ld + last) * 2;
       step = (KS ? BK * ld : BK) * 2;
       left = k_end - k0;
@@ -552,7 +553,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 1) void
   write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, buf + wave * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
 }
 
-// Operands of 16-bit types on 16-byte boundaries: tiles of 32 k go straight from memory into a ring of four LDS buffers, with one
+// Operands of 16-bit types whose rows are whole 16-byte pieces on 16-byte boundaries (with zeros in the last piece behind the
+// last k, where k runs along the row): tiles of 32 k go straight from memory into a ring of four LDS buffers, with one
 // barrier a step: it tells that a tile has landed for every wavefront (each waits for its own part) and that nobody reads
 // the oldest one any more, whose buffer is then filled again.
 // While step t is multiplied, tiles t+2 and t+3 are on their way and t+1 is there, so that its first fragments are read before

@@ -24,6 +24,8 @@ def _ptr(t):
 def _as_rows(t):
     """t as [rows, last dimension] whose last dimension is contiguous: (tensor, row stride)."""
     n = t.shape[-1]
+    if t.is_contiguous():
+        return (t if t.dim() == 2 else t.view(-1, n)), n
     if t.dim() != 2:
         t = t.reshape(-1, n)
     if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n):
@@ -76,8 +78,9 @@ class _LayerFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("dense: the gradient is not differentiable (create_graph)")
         x, kernel, y, aux, offset_t = ctx.saved_tensors
         need_x, need_k, need_b, need_r = ctx.needs_input_grad[:4]
         d_residual = dy if need_r else None

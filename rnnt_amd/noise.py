@@ -10,28 +10,23 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._operator import check, drop16, dtype_code, need_gpu, on_device, seed_offset, stream
-
-
-def _rows(x):
-    """x as rows of its last dimension: (tensor to read, rows, columns, row stride).  One-dimensional rows may be any
-    distance apart; anything else is made dense."""
-    cols = x.shape[-1]
-    if x.dim() == 1:
-        return (x if x.stride(0) == 1 else x.contiguous()), 1, cols, cols
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
-        return x, x.shape[0], cols, x.stride(0)
-    x = x.contiguous()
-    return x, x.numel() // cols, cols, cols
+from ._operator import DTYPE_CODE, check, drop16, dtype_code, need_gpu, on_device, seed_offset, stream
 
 
 def _apply(x, drop, seed, offset, offset_t):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    x, rows, cols, stride = _rows(x)
+    cols = stride = x.shape[-1]
+    if not x.is_contiguous():
+        # rows of a matrix may be any distance apart; anything else is made dense
+        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+            stride = x.stride(0)
+        else:
+            x = x.contiguous()
     with on_device(x.device):
-        rc = _lib.lib().rnnt_mi355x_dropout(x.data_ptr(), stride, y.data_ptr(), rows, cols, dtype_code("dropout", x), drop, seed, offset,
+        rc = _lib.lib().rnnt_mi355x_dropout(x.data_ptr(), stride, y.data_ptr(), x.numel() // cols, cols, DTYPE_CODE[x.dtype], drop, seed, offset,
                                             None if offset_t is None else offset_t.data_ptr(), stream(x.device))
-    check(rc, "rnnt_mi355x_dropout")
+    if rc:
+        check(rc, "rnnt_mi355x_dropout")
     return y
 
 
@@ -39,14 +34,17 @@ class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, drop, seed, offset, offset_t):
         ctx.args = (drop, seed, offset)
-        ctx.save_for_backward(offset_t)  # its version is checked: the backward pass needs the same offset
+        if offset_t is not None:
+            ctx.save_for_backward(offset_t)  # its version is checked: the backward pass needs the same offset
+        ctx.has_offset = offset_t is not None
         return _apply(x, drop, seed, offset, offset_t)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        (offset_t,) = ctx.saved_tensors
-        return _apply(dy, *ctx.args, offset_t), None, None, None, None
+        args = (*ctx.args, ctx.saved_tensors[0] if ctx.has_offset else None)
+        if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same linear map again
+            return _DropoutFn.apply(dy, *args), None, None, None, None
+        return _apply(dy, *args), None, None, None, None
 
 
 def dropout(x, rate, seed=0, offset=0):

@@ -88,7 +88,8 @@ def check_layer(M, K, N, dtype, act="linear", bias=True, residual=False, rate=0.
 
 
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (8, 250, 62), (31, 33, 40), (32, 64, 128), (33, 64, 72), (64, 520, 136), (65, 129, 66),
-          (100, 1000, 65), (130, 96, 130), (257, 72, 264), (300, 515, 103), (129, 2056, 136), (1000, 40, 250)]
+          (100, 1000, 65), (130, 96, 130), (257, 72, 264), (300, 515, 103), (129, 2056, 136), (1000, 40, 250),
+          (600, 515, 1030), (513, 77, 33), (520, 64, 65), (777, 1003, 130)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -270,6 +271,26 @@ def test_streams_and_graphs():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(out, step()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 5000, 300), (2, 1030, 65), (3, 77, 1001), (4, 512, 513), (7, 1024, 64), (8, 2500, 130), (8, 4096, 20000)])
+def test_few_rows(M, K, N, dtype):
+    """The decoder's form: no gradients, every epilogue."""
+    x, w, b, r, _ = data(M, K, N, dtype, 11, residual=True)
+    y = rnnt_amd.dense(x.to(DEV), w.to(DEV), b.to(DEV), "silu", r.to(DEV), 0.2, 3, 4)
+    X, W = f64(x), f64(w)
+    scale = orc.dropout_scale(M, N, 0.2, 3, 4)
+    z = X @ W + f64(b)
+    want = orc.activation(z, "silu")[0] * scale + f64(r)
+    ey = scale * (1.13 * acc(K, np.abs(X) @ np.abs(W) + np.abs(f64(b))) + 2.0 ** -21 * (1 + np.abs(z))) + 2.0 ** -23 * (np.abs(want) + np.abs(f64(r)))
+    assert (np.abs(f64(y) - want) <= ey + np.maximum(U[dtype] * (np.abs(want) + ey), LEAST[dtype])).all()
+
+
+def test_gradient_of_the_gradient_is_refused():
+    x, w = torch.ones(4, 8, device=DEV, requires_grad=True), torch.ones(8, 6, device=DEV)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(rnnt_amd.dense(x, w, activation="gelu").sum(), x, create_graph=True)
 
 
 def test_refusals():

@@ -112,6 +112,14 @@ def test_backward_refuses_an_offset_that_has_moved():
         y.sum().backward()
 
 
+def test_gradient_of_the_gradient():
+    x = torch.randn(5, 9, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad((rnnt_amd.dropout(x, 0.5, seed=3) ** 2).sum(), x, create_graph=True)
+    (gg,) = torch.autograd.grad(g.sum(), x)
+    scale = torch.from_numpy(orc.dropout_scale(5, 9, 0.5, 3, 0)).to(DEV)
+    assert torch.equal(gg.double(), 2 * scale ** 2)
+
+
 def test_refusals():
     x = torch.zeros(3, 4, device=DEV)
     with pytest.raises(TypeError):
