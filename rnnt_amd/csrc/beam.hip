@@ -10,7 +10,7 @@
 // softmax sum; the totals themselves are formed in float64, because candidates of different beams lie arbitrarily close
 // and a float32 sum would order them by its rounding.
 //   - the lanes' maxima are sorted across the wavefront; the width-th of them is a lower bound T of the width-th largest
-//     value, and the few values >= T are compacted and sorted (64 at a time, a bitonic network over the lanes);
+//     value, and the few values >= T are compacted and sorted (a bitonic network over the lanes);
 //   - sorted lists are joined by the first step of a bitonic merge: of two sorted lists a, b the values
 //     max(a[i], b[P-1-i]) are the P largest, and log2 P exchanges sort them.
 // Rows of up to 2048 symbols take one launch, a block per utterance; longer ones a launch over pieces of 2048 and one that
@@ -20,8 +20,6 @@
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLog2eLow = 1.925963033500924e-8f;  // log2 e - (float)log2 e
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kScoreLimit = 1073741824.f;  // 2^30: a score beyond it marks an empty beam (or is no score at all)
 constexpr int kMaxBeams = 64, kMaxWidth = 64;
 constexpr int kPiece = 2048;  // symbols of a row that one wavefront takes
@@ -36,7 +34,17 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
   else if constexpr (M == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);  // row_ror:8
   else if constexpr (M == 15) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true); // row_mirror
   else if constexpr (M == 4) return lane_xor<7>(lane_xor<3>(v));
-  else return __shfl_xor(v, M, 64);
+  else if constexpr (M == 16) {  // the first result has rows 0, 0, 2, 2 of 16 lanes, the second 1, 1, 3, 3
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else if constexpr (M == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  } else if constexpr (M == 31) return lane_xor<16>(lane_xor<15>(v));
+  else {
+    static_assert(M == 63, "");
+    return lane_xor<32>(lane_xor<16>(lane_xor<15>(v)));
+  }
 }
 
 // Candidates: larger is better, all of them different; zero stands for none.
@@ -106,15 +114,31 @@ __device__ __forceinline__ void join(K& acc, const K& reversed, int lane) {
   clean<P>(acc, lane);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+template <int M>
+__device__ __forceinline__ float lane_xor(float v) {
+  return __uint_as_float(lane_xor<M>(__float_as_uint(v)));
 }
+template <int M>
+__device__ __forceinline__ double lane_xor(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, ((uint64_t)lane_xor<M>((uint32_t)(b >> 32)) << 32) | lane_xor<M>((uint32_t)b));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, lane_xor<1>(v));
+  v = fmaxf(v, lane_xor<2>(v));
+  v = fmaxf(v, lane_xor<7>(v));
+  v = fmaxf(v, lane_xor<15>(v));
+  v = fmaxf(v, lane_xor<16>(v));
+  return fmaxf(v, lane_xor<32>(v));
+}
+// the same order of additions in every wavefront: equal rows get equal sums
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  v += lane_xor<1>(v);
+  v += lane_xor<2>(v);
+  v += lane_xor<7>(v);
+  v += lane_xor<15>(v);
+  v += lane_xor<16>(v);
+  return v + lane_xor<32>(v);
 }
 
 // What a wavefront's lanes wrote to LDS is there for its other lanes.
@@ -181,77 +205,113 @@ __device__ __forceinline__ void load_piece(const BeamArgs& a, int b, int k, int 
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[8 * j + i] = y[i] + 0.f;  // -0 becomes +0: the two tie
+    for (int i = 0; i < 8; ++i) x[8 * j + i] = y[i];
   }
 }
 
+// 64 values in descending order over the lanes, without what they belong to.
+template <int M, int D>
+__device__ __forceinline__ void exchange_value(uint32_t& v, int lane) {
+  const uint32_t o = lane_xor<M>(v);
+  v = lane & D ? min(v, o) : max(v, o);
+}
+__device__ __forceinline__ void sort64_values(uint32_t& v, int lane) {
+  exchange_value<1, 1>(v, lane);
+  exchange_value<3, 2>(v, lane);
+  exchange_value<1, 1>(v, lane);
+  exchange_value<7, 4>(v, lane);
+  exchange_value<2, 2>(v, lane);
+  exchange_value<1, 1>(v, lane);
+  exchange_value<15, 8>(v, lane);
+  exchange_value<4, 4>(v, lane);
+  exchange_value<2, 2>(v, lane);
+  exchange_value<1, 1>(v, lane);
+  exchange_value<31, 16>(v, lane);
+  exchange_value<8, 8>(v, lane);
+  exchange_value<4, 4>(v, lane);
+  exchange_value<2, 2>(v, lane);
+  exchange_value<1, 1>(v, lane);
+  exchange_value<63, 32>(v, lane);
+  exchange_value<16, 16>(v, lane);
+  exchange_value<8, 8>(v, lane);
+  exchange_value<4, 4>(v, lane);
+  exchange_value<2, 2>(v, lane);
+  exchange_value<1, 1>(v, lane);
+}
+
+// The larger of a lane's key and its partner's.
+template <int M>
+__device__ __forceinline__ RowKey larger(const RowKey& k) {
+  const RowKey o = lane_xor<M>(k);
+  return o > k ? o : k;
+}
+
 // Softmax share and the 64 best candidates of a piece: *m the largest value, *s = sum exp(x - m) (NaN when a value is NaN
-// or +inf), and in lane i the i-th candidate, of which the first `width` are right.  buf: 128 keys of LDS of this wavefront.
+// or +inf), and in lane i the i-th candidate, of which the first `width` are right.  buf: 64 keys of LDS of this wavefront.
 template <int E>
 __device__ __forceinline__ RowKey best_of_piece(const float (&x)[E], int v0, int width, int lane, RowKey* buf, float* m, double* s) {
-  float top = -INFINITY;
-  int at = 0;
+  float top = x[0];
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (x[e] > top) {
-      top = x[e];
-      at = (e >> 3) * 512 + lane * 8 + (e & 7);
-    }
-  const float mx = wave_max(top);
-  const float base = mx == -INFINITY ? 0.f : mx;
+  for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);  // drops NaN, which the sum keeps
+  if (top != top) top = -INFINITY;
+  const float mx = wave_max(top), base = mx == -INFINITY ? 0.f : mx;
+  // Eight float32 terms pairwise, then float64: the sum decides between candidates of different beams.  A term is off by
+  // about 2^-23 of itself, at random; over a row that leaves some 10^-8 of the sum.
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    // exp(x - m) to about one unit in the last place: the difference and its product with log2 e with their rounding
-    // errors (the sum decides between candidates of different beams)
-    const float d = x[e] - base, bb = d - x[e], err = (x[e] - (d - bb)) - (base + bb);
-    const float t = d * kLog2e;
-    const float low = fmaf(err, kLog2e, fmaf(d, kLog2eLow, fmaf(d, kLog2e, -t)));
-    const float p = __builtin_amdgcn_exp2f(t);
-    // below 2^-160 the term is zero, also where x = -inf or the difference overflows and the corrections are NaN; a NaN
-    // among the values stays one
-    const float term = t < -160.f ? 0.f : fmaf(p * kLn2, low, p);
-    sum += (double)term;
+  for (int e = 0; e < E; e += 8) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f((x[e + i] - base) * kLog2e);  // 2^-inf = 0
+    sum += (double)(((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
   }
   *m = mx;
   *s = wave_sum(sum);
 
-  RowKey lanes = {0u, 0u};
-  if (top > -INFINITY) lanes = {ordered(top), ~(uint32_t)(v0 + at)};
-  sort64(lanes, lane);
-  const RowKey bound = {(uint32_t)__shfl((int)lanes.hi, width - 1, 64), (uint32_t)__shfl((int)lanes.lo, width - 1, 64)};
-  const float floor_x = bound.hi ? unordered(bound.hi) : -INFINITY;
-  RowKey acc = {0u, 0u};
+  // `width` lanes have a value of floor_x or more
+  uint32_t tops = top > -INFINITY ? ordered(top + 0.f) : 0u;
+  sort64_values(tops, lane);
+  const uint32_t floor_key = (uint32_t)__shfl((int)tops, width - 1, 64);
+  const float floor_x = floor_key ? unordered(floor_key) : -__FLT_MAX__;  // -inf is never a candidate
+  auto place = [&](int e) { return (uint32_t)(v0 + (e >> 3) * 512 + lane * 8 + (e & 7)); };
   int fill = 0;
-  bool first = true;
-  auto take = [&](int n) {  // the first n <= 64 keys of the buffer join acc
-    wave_sync();
-    RowKey k = {0u, 0u};
-    if (lane < n) k = buf[lane];
-    sort64(k, lane);
-    if (first) acc = k;
-    else join<64>(acc, lane_xor<63>(k), lane);
-    first = false;
-  };
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const RowKey k = {ordered(x[e]), ~(uint32_t)(v0 + (e >> 3) * 512 + lane * 8 + (e & 7))};
-    const bool in = x[e] >= floor_x && x[e] > -INFINITY && !(bound > k);
+    const bool in = x[e] >= floor_x;
     const uint64_t who = __ballot(in);
     if (who) {  // uniform
-      if (in) buf[fill + __popcll(who & ((1ull << lane) - 1))] = k;
+      const int at = fill + __popcll(who & ((1ull << lane) - 1));
+      if (in && at < 64) buf[at] = RowKey{__float_as_uint(x[e]), place(e)};
       fill += __popcll(who);
-      if (fill >= 64) {
-        take(64);
-        RowKey rest = {0u, 0u};
-        if (lane < fill - 64) rest = buf[64 + lane];
-        wave_sync();
-        if (lane < fill - 64) buf[lane] = rest;
-        fill -= 64;
-      }
     }
   }
-  if (fill > 0) take(fill);
+  RowKey acc = {0u, 0u};
+  if (fill <= 64) {  // uniform, and nearly always so
+    wave_sync();
+    if (lane < fill) acc = RowKey{ordered(__uint_as_float(buf[lane].hi) + 0.f), ~buf[lane].lo};  // -0 and +0 tie
+    sort64(acc, lane);
+    return acc;
+  }
+  // Many values of one size, or many of the best in one lane: the next best key of all, `width` times over.
+  RowKey last = {~0u, ~0u};
+#pragma unroll 1
+  for (int i = 0; i < width; ++i) {
+    RowKey best = {0u, 0u};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const RowKey k = {x[e] >= floor_x ? ordered(x[e] + 0.f) : 0u, ~place(e)};
+      if (last > k && k > best) best = k;
+    }
+    if (best.hi == 0u) best.lo = 0u;
+    best = larger<1>(best);
+    best = larger<2>(best);
+    best = larger<7>(best);
+    best = larger<15>(best);
+    best = larger<16>(best);
+    best = larger<32>(best);
+    if (lane == i) acc = best;
+    last = best;
+  }
   return acc;
 }
 
@@ -300,14 +360,14 @@ __device__ __forceinline__ void join_block(TotalKey& acc, TotalKey (*lds)[64], i
 }
 
 // One launch for short rows: a block per utterance, its wavefronts share the beams.
-// 32 values a lane, with what they are loaded into, do not fit the 128 registers of 16 wavefronts: such blocks have 8.
+// More than 8 values a lane, with what they are loaded into, do not fit the 128 registers of 16 wavefronts: such blocks have 8.
 template <class T, int E, int P>
-__global__ __launch_bounds__(E == 32 ? 512 : 1024) void k_beam_rows(BeamArgs a) {
+__global__ __launch_bounds__(E > 8 ? 512 : 1024) void k_beam_rows(BeamArgs a) {
   __shared__ RowKey lists[kMaxBeams][P];
   __shared__ RowSum rows[kMaxBeams];
   __shared__ TotalKey tree[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
-  RowKey* buf = reinterpret_cast<RowKey*>(tree[wave]);  // 128 keys; the lists are joined there after the barrier
+  RowKey* buf = reinterpret_cast<RowKey*>(tree[wave]);  // 64 keys; the lists are joined there after the barrier
   for (int k = wave; k < a.K; k += waves) {
     const float score = a.scores[(long long)b * a.K + k];
     const bool done = a.finished && a.finished[(long long)b * a.K + k];
@@ -350,28 +410,33 @@ struct PieceSum {
 };
 template <class T, int P>
 __global__ __launch_bounds__(256) void k_beam_pieces(BeamArgs a, PieceSum* sums, RowKey* lists) {
-  __shared__ RowKey buf[4][128];
+  __shared__ RowKey buf[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long id = (long long)blockIdx.x * 4 + wave;
-  if (id >= (long long)a.B * a.K * a.pieces) return;
-  const int piece = (int)(id % a.pieces);
-  const long long row = id / a.pieces;
+  const unsigned id = blockIdx.x * 4u + (unsigned)__builtin_amdgcn_readfirstlane(wave);  // B * K * pieces < 2^31
+  if (id >= (unsigned)a.B * (unsigned)a.K * (unsigned)a.pieces) return;
+  const unsigned row = id / (unsigned)a.pieces;
+  const int piece = (int)(id - row * (unsigned)a.pieces);
   if (!live_score(a.scores[row]) || (a.finished && a.finished[row])) return;  // nothing of it is read
   float x[kPiece / 64], m;
   double s;
-  load_piece<T, kPiece / 64>(a, (int)(row / a.K), (int)(row % a.K), piece * kPiece, lane, x);
+  load_piece<T, kPiece / 64>(a, (int)(row / (unsigned)a.K), (int)(row % (unsigned)a.K), piece * kPiece, lane, x);
   const RowKey best = best_of_piece<kPiece / 64>(x, piece * kPiece, a.width, lane, buf[wave], &m, &s);
-  if (lane < P) lists[id * P + lane] = lane < a.width ? best : RowKey{0u, 0u};
+  if (lane < P) lists[(long long)id * P + lane] = lane < a.width ? best : RowKey{0u, 0u};
   if (lane == 0) sums[id] = PieceSum{s, m, 0.f};
 }
 
-// Second launch: a block per utterance joins the pieces.
+// Second launch: a block per utterance joins the pieces.  Only the `width` lists with the best first entries can hold
+// anything that is kept: the first entries alone choose them, and only those lists are read on.
 template <int P>
 __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* sums, const RowKey* lists) {
   __shared__ RowSum rows[kMaxBeams];
   __shared__ float live[kMaxBeams];  // the score of a beam that has candidates, else NaN
+  __shared__ bool over[kMaxBeams];   // finished: its score is its one candidate
   __shared__ TotalKey tree[16][64];
+  __shared__ TotalKey best[kMaxWidth];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
+  const int lists_here = a.K * a.pieces;
+  lists += (long long)b * lists_here * P;
   for (int k = wave; k < a.K; k += waves) {
     const long long row = (long long)b * a.K + k;
     float score = a.scores[row];
@@ -395,29 +460,41 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
     if (lane == 0) {
       rows[k] = of;
       live[k] = score;
+      over[k] = done;
     }
   }
   __syncthreads();
+  auto entry = [&](int l, int r) {  // the r-th candidate of list l
+    const int k = l / a.pieces;
+    const float score = live[k];
+    if (score != score) return TotalKey{0ull, 0u};
+    if (!over[k]) return total_key(a, k, false, score, rows[k], lists[(long long)l * P + r]);
+    return r == 0 && l == k * a.pieces ? total_key(a, k, true, score, rows[k], RowKey{0u, 0u}) : TotalKey{0ull, 0u};
+  };
+  TotalKey heads = {0ull, 0u};
+  for (int l0 = wave * 64; l0 < lists_here; l0 += waves * 64) {
+    TotalKey t = {0ull, 0u};
+    if (l0 + lane < lists_here) t = entry(l0 + lane, 0);
+    if (__any(t.hi != 0)) {
+      sort64(t, lane);
+      join<64>(heads, lane_xor<63>(t), lane);
+    }
+  }
+  join_block<64>(heads, tree, wave, waves, lane);
+  if (wave == 0 && lane < a.width) best[lane] = heads;
+  __syncthreads();
+
   TotalKey acc = {0ull, 0u};
   constexpr int G = 64 / P;
   const int i = lane & (P - 1), r = P - 1 - i;
-  const int lists_here = a.K * a.pieces;
-  for (int l0 = wave * G; l0 < lists_here; l0 += waves * G) {
-    const int l = l0 + lane / P;
+  for (int l0 = wave * G; l0 < a.width; l0 += waves * G) {
     TotalKey t = {0ull, 0u};
-    if (l < lists_here) {
-      const int k = l / a.pieces, piece = l - k * a.pieces;
-      const float score = live[k];
-      const bool done = a.finished && a.finished[(long long)b * a.K + k];
-      if (score == score) {
-        if (done) {
-          if (piece == 0 && r == 0) t = total_key(a, k, true, score, rows[k], RowKey{0u, 0u});
-        } else {
-          t = total_key(a, k, false, score, rows[k], lists[((long long)b * lists_here + l) * P + r]);
-        }
-      }
+    const int w = l0 + lane / P;
+    if (w < a.width && best[w].hi) {
+      const uint32_t flat = ~best[w].lo, k = flat / (uint32_t)a.V;
+      t = entry((int)k * a.pieces + (over[k] ? 0 : (int)(flat - k * (uint32_t)a.V) / kPiece), r);
     }
-    if (__any(t > acc)) join<P>(acc, t, lane);  // lists that hold nothing better than the last of acc change nothing
+    join<P>(acc, t, lane);
   }
   join_block<P>(acc, tree, wave, waves, lane);
   if (wave == 0) write_out(a, b, lane, acc);
@@ -434,7 +511,7 @@ int pow2_up(int v) {
 template <class T, int P>
 int launch_select(const BeamArgs& a, void* workspace, hipStream_t st) {
   if (a.pieces == 0) {
-    const int most = a.V <= 1024 ? 16 : 8, waves = a.K >= most ? most : pow2_up(a.K);
+    const int most = a.V <= 512 ? 16 : 8, waves = a.K >= most ? most : pow2_up(a.K);
     if (a.V <= 512) k_beam_rows<T, 8, P><<<a.B, waves * 64, 0, st>>>(a);
     else if (a.V <= 1024) k_beam_rows<T, 16, P><<<a.B, waves * 64, 0, st>>>(a);
     else k_beam_rows<T, 32, P><<<a.B, waves * 64, 0, st>>>(a);
@@ -444,7 +521,7 @@ int launch_select(const BeamArgs& a, void* workspace, hipStream_t st) {
     RowKey* lists = reinterpret_cast<RowKey*>(sums + n);
     k_beam_pieces<T, P><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(a, sums, lists);
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
-    const int waves = min(16, pow2_up((a.K * a.pieces * P + 63) / 64));
+    const int waves = min(16, max(pow2_up((a.K * a.pieces + 63) / 64), pow2_up((a.width * P + 63) / 64)));
     k_beam_join<P><<<a.B, waves * 64, 0, st>>>(a, sums, lists);
   }
   return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
