@@ -46,7 +46,7 @@ REORDER_MAX = 16  # RNNT_MI355X_REORDER_MAX
 
 
 class ReorderTensor(ctypes.Structure):
-    """rnnt_mi355x_reorder_tensor"""
+    """rnnt_mi355x_reorder_tensor; its fields are eight bytes each, so a table of them is also an array of integers"""
     _fields_ = [("src", _vp), ("dst", _vp)] + [(n, _ll) for n in ("outer", "outer_stride", "batch_stride", "beam_stride", "row_bytes")]
 
 
@@ -89,7 +89,7 @@ _SIGNATURES = {
     "rnnt_mi355x_layer_backward": (ctypes.c_int, [ctypes.POINTER(Layer), _vp, _ll] + [_vp] * 5),
     "rnnt_mi355x_beam_select_workspace_bytes": (ctypes.c_int, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "rnnt_mi355x_beam_select": (ctypes.c_int, [_vp, _ll, _ll, _i, _vp, _ll, _vp, _vp, _ll, _vp] + [_i] * 5 + [_vp] * 5),
-    "rnnt_mi355x_beam_reorder": (ctypes.c_int, [ctypes.POINTER(ReorderTensor), _i, _vp, _i, _i, _i, _vp]),
+    "rnnt_mi355x_beam_reorder": (ctypes.c_int, [_vp, _i, _vp, _i, _i, _i, _vp]),
     "rnnt_mi355x_reduce_scalars": (ctypes.c_int, [_vp, _i, _vp, _vp, _vp]),
     "rnnt_mi355x_read_status": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int32), _vp]),
     "rnnt_mi355x_status_string": (ctypes.c_char_p, [_i]),

@@ -47,12 +47,15 @@ def need_gpu(what: str, **tensors):
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} must be a tensor")
-        if t.device.type != "cuda":
-            raise ValueError(f"{what}: {name} must live on an MI355X device (there is no CPU path)")
+        d = t.device
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: {name} lives on {t.device}, the others on {dev}")
+            if d.type != "cuda":
+                raise ValueError(f"{what}: {name} must live on an MI355X device (there is no CPU path)")
+            dev = d
+        elif d != dev:
+            if d.type != "cuda":
+                raise ValueError(f"{what}: {name} must live on an MI355X device (there is no CPU path)")
+            raise ValueError(f"{what}: {name} lives on {d}, the others on {dev}")
     return dev
 
 

@@ -51,30 +51,37 @@ def beam_select(logits, scores, width, enc=None, allowed=None, finished=None, en
             raise ValueError("beam_select: finished must be bool [B, K]")
         if not 0 <= int(end) < V:
             raise ValueError(f"beam_select: end {end} outside [0, {V})")
-    if V > 1 and logits.stride(2) != 1:
+    s0, s1, s2 = logits.stride()
+    if s2 != 1 and V > 1:
         logits = logits.contiguous()
-    if enc is not None and V > 1 and enc.stride(1) != 1:
-        enc = enc.contiguous()
-    if allowed is not None and V > 1 and allowed.stride(-1) != 1:
-        allowed = allowed.contiguous()
+        s0, s1, s2 = logits.stride()
+    enc_p = enc_s = allowed_p = allowed_s = fin_p = ws_p = 0
+    if enc is not None:
+        if V > 1 and enc.stride(1) != 1:
+            enc = enc.contiguous()
+        enc_p, enc_s = enc.data_ptr(), enc.stride(0)
+    if allowed is not None:
+        if V > 1 and allowed.stride(-1) != 1:
+            allowed = allowed.contiguous()
+        allowed_p, allowed_s = allowed.data_ptr(), allowed.stride(0) if allowed.dim() == 2 else 0
+    if finished is not None:
+        finished = finished.contiguous()
+        fin_p = finished.data_ptr()
     scores = scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
     out = torch.empty((3, B, width), dtype=torch.int32, device=dev)
     out_scores, parent, token = out.unbind(0)
     L = _lib.lib()
     with on_device(dev):
-        ws = None
-        if V > 2048:  # rows of one piece need none
+        if V > 2048:  # rows of one piece need no workspace
             n = ctypes.c_size_t(0)
             check(L.rnnt_mi355x_beam_select_workspace_bytes(B, K, V, width, ctypes.byref(n)), "rnnt_mi355x_beam_select_workspace_bytes")
             ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        rc = L.rnnt_mi355x_beam_select(logits.data_ptr(), logits.stride(0), logits.stride(1), code, None if enc is None else enc.data_ptr(),
-                                       0 if enc is None else enc.stride(0), scores.data_ptr(), None if allowed is None else allowed.data_ptr(),
-                                       allowed.stride(0) if allowed is not None and allowed.dim() == 2 else 0,
-                                       None if finished is None else finished.data_ptr(), int(end) if finished is not None else 0, B, K, V, width,
-                                       out_scores.data_ptr(), parent.data_ptr(), token.data_ptr(), None if ws is None else ws.data_ptr(),
-                                       stream(dev))
-    check(rc, "rnnt_mi355x_beam_select")
+            ws_p = ws.data_ptr()
+        o, step = out.data_ptr(), 4 * B * width
+        rc = L.rnnt_mi355x_beam_select(logits.data_ptr(), s0, s1, code, enc_p, enc_s, scores.data_ptr(), allowed_p, allowed_s, fin_p,
+                                       int(end) if fin_p else 0, B, K, V, width, o, o + step, o + 2 * step, ws_p, stream(dev))
+    if rc:
+        check(rc, "rnnt_mi355x_beam_select")
     return out_scores.view(torch.float32), parent, token
 
 
@@ -95,15 +102,14 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
         raise ValueError("beam_reorder: parent must be int32 [B, W]")
     states = list(states)
     dev = need_gpu("beam_reorder", parent=parent)
-    for i, s in enumerate(states):
-        if not isinstance(s, torch.Tensor) or s.device != dev:
-            need_gpu("beam_reorder", parent=parent, **{f"states[{i}]": s})
+    if any(not isinstance(s, torch.Tensor) or s.device != dev for s in states):
+        need_gpu("beam_reorder", parent=parent, **{f"states[{i}]": s for i, s in enumerate(states)})
     B, W = parent.shape
     d = int(batch_dim)
     if d < 0:
         raise ValueError("beam_reorder: batch_dim counts from the first dimension")
     K = -1
-    new, todo, keep = [], [], [parent if parent.is_contiguous() else parent.contiguous()]
+    new = []
     for i, s in enumerate(states):
         shape = s.shape
         if len(shape) < d + 2 or shape[d] != B:
@@ -128,19 +134,25 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
         for o in out:
             o.zero_()
         return out
+    if not parent.is_contiguous():
+        parent = parent.contiguous()
+    table, keep = [], []  # the fields of rnnt_mi355x_reorder_tensor, one tensor after the other
     for s, o in zip(states, out):
-        if o.numel() == 0:
+        n = o.numel()
+        if n == 0:
             continue
         # [outer, B, K, row]: the row has to be dense, the three leading dimensions need one stride each
         if not s.is_contiguous() and (d > 1 or not s[(0,) * (d + 2)].is_contiguous()):
             s = s.contiguous()
             keep.append(s)
         e, strides = s.element_size(), s.stride()
-        row, outer = math.prod(s.shape[d + 2:]), math.prod(s.shape[:d])
-        todo.append(_lib.ReorderTensor(s.data_ptr(), o.data_ptr(), outer, strides[d - 1] * e if d else 0, strides[d] * e, strides[d + 1] * e, row * e))
+        outer = s.shape[0] if d == 1 else math.prod(s.shape[:d])
+        table += (s.data_ptr(), o.data_ptr(), outer, strides[d - 1] * e if d else 0, strides[d] * e, strides[d + 1] * e, n // (outer * B * W) * e)
+    f, most = _lib.lib().rnnt_mi355x_beam_reorder, 7 * _lib.REORDER_MAX
     with on_device(dev):
-        for i in range(0, len(todo), _lib.REORDER_MAX):
-            part = todo[i:i + _lib.REORDER_MAX]
-            rc = _lib.lib().rnnt_mi355x_beam_reorder((_lib.ReorderTensor * len(part))(*part), len(part), keep[0].data_ptr(), B, K, W, stream(dev))
-            check(rc, "rnnt_mi355x_beam_reorder")
+        for i in range(0, len(table), most):
+            part = table[i:i + most]
+            rc = f((ctypes.c_longlong * len(part))(*part), len(part) // 7, parent.data_ptr(), B, K, W, stream(dev))
+            if rc:
+                check(rc, "rnnt_mi355x_beam_reorder")
     return out

@@ -19,6 +19,8 @@ struct DzArgs {
   float* partial;   // nullable [row blocks][N]
   long long dy_ld, dz_ld;
   int M, N, rows;   // rows of a block
+  int across;       // blocks that a row takes
+  unsigned blocks;  // of this pass; copies follow
   int act, from;
   DropArgs drop;
 };
@@ -63,14 +65,46 @@ __device__ __forceinline__ void slopes8(const DzArgs& a, long long m, int n0, in
   }
 }
 
-// Bound by memory: dy and the saved tensor read once, dz written once.
+// ---- rows that do not lie on 16-byte boundaries --------------------------------------------------------------------------
+// A 16-bit matrix copied to rows of whole 16-byte pieces, zeros behind the last column: with it the products take the
+// ring kernel.
+struct PackArgs {
+  const uint16_t* src;
+  uint16_t* dst;
+  long long src_ld, dst_ld, rows;
+  int cols;
+  unsigned blocks;  // 0: nothing to copy
+};
+__device__ __forceinline__ void pack_block(const PackArgs& p, unsigned block) {
+  const int pieces = (p.cols + 7) / 8;
+  const long long id = (long long)block * 256 + threadIdx.x, row = id / pieces;
+  if (row >= p.rows) return;
+  const int c = (int)(id - row * pieces) * 8;
+  const Raw8<Bf16> r = load_group<Bf16>(p.src + row * p.src_ld + c, p.cols - c);
+  *reinterpret_cast<u4*>(p.dst + row * p.dst_ld + c) = r.q[0];
+}
+__global__ __launch_bounds__(256) void k_layer_pack(PackArgs a, PackArgs b) {
+  if (blockIdx.x < a.blocks) pack_block(a, blockIdx.x);
+  else pack_block(b, blockIdx.x - a.blocks);
+}
+
+// dz, its column sums, and the copies of the operands that lie badly: what the gradient's products begin with.  Bound by
+// memory: dy and the saved tensor read once, dz written once.
 template <class T>
-__global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a) {
+__global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a, PackArgs p, PackArgs q) {
+  static_assert(kDzGroups * kDzLanes == 256, "pack_block's size");
   __shared__ float sums[kDzLanes][kDzGroups * 8 + 4];
+  if (blockIdx.x >= a.blocks) {
+    const unsigned i = blockIdx.x - a.blocks;
+    if (i < p.blocks) pack_block(p, i);
+    else pack_block(q, i - p.blocks);
+    return;
+  }
   load_offset(a.drop);
+  const int bx = blockIdx.x % (unsigned)a.across, by = blockIdx.x / (unsigned)a.across;
   const int gx = threadIdx.x % kDzGroups, ty = threadIdx.x / kDzGroups;
-  const int n0 = (blockIdx.x * kDzGroups + gx) * 8, left = a.N - n0;
-  const int m0 = blockIdx.y * a.rows, m1 = min(a.M, m0 + a.rows);
+  const int n0 = (bx * kDzGroups + gx) * 8, left = a.N - n0;
+  const int m0 = by * a.rows, m1 = min(a.M, m0 + a.rows);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (left > 0) {
 #pragma unroll 2
@@ -93,61 +127,50 @@ __global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[ty][gx * 8 + i] = sum[i];
   __syncthreads();
-  const int n = blockIdx.x * kDzGroups * 8 + threadIdx.x;
+  const int n = bx * kDzGroups * 8 + threadIdx.x;
   if (n < a.N) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < kDzLanes; ++i) s += sums[i][threadIdx.x];
-    a.partial[(long long)blockIdx.y * a.N + n] = s;
+    a.partial[(long long)by * a.N + n] = s;
   }
 }
 
-// db: the row blocks' sums, 32 columns and 32 blocks at a time; the order is fixed.
-template <class T>
-__global__ __launch_bounds__(1024) void k_layer_db(const float* partial, int blocks, int N, typename T::elem* db) {
-  __shared__ float sums[32][33];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
-  float s = 0.f;
-  if (n < N) {
-#pragma unroll 8
-    for (int i = r; i < blocks; i += 32) s += partial[(long long)i * N + n];
-  }
-  sums[r][c] = s;
-  __syncthreads();
-  if (r == 0 && n < N) {
-#pragma unroll
-    for (int i = 1; i < 32; ++i) s += sums[i][c];
-    db[n] = from_float<T>(s);
-  }
-}
-
-// ---- rows that do not lie on 16-byte boundaries --------------------------------------------------------------------------
-// A 16-bit matrix copied to rows of whole 16-byte pieces, zeros behind the last column: with it the products take the
-// ring kernel.
-struct PackArgs {
-  const uint16_t* src;
-  uint16_t* dst;
-  long long src_ld, dst_ld, rows;
-  int cols;
+// ---- joining the splits of a product, and db from its partial sums -------------------------------------------------------
+struct DbArgs {
+  const float* partial;  // [blocks][N]
+  void* db;              // null: none
+  int blocks, N;
 };
-__global__ __launch_bounds__(256) void k_layer_pack(PackArgs a, PackArgs b, unsigned a_blocks) {
-  const PackArgs p = blockIdx.x < a_blocks ? a : b;
-  const long long block = blockIdx.x < a_blocks ? blockIdx.x : blockIdx.x - a_blocks;
-  const int pieces = (p.cols + 7) / 8;
-  const long long id = block * 256 + threadIdx.x, row = id / pieces;
-  if (row >= p.rows) return;
-  const int c = (int)(id - row * pieces) * 8;
-  const Raw8<Bf16> r = load_group<Bf16>(p.src + row * p.src_ld + c, p.cols - c);
-  *reinterpret_cast<u4*>(p.dst + row * p.dst_ld + c) = r.q[0];
+// 16 columns, 16 row blocks at a time; the order is fixed
+template <class T>
+__device__ __forceinline__ void db_block(const DbArgs& d, unsigned block, float* sums) {
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = block * 16 + c;
+  float s = 0.f;
+  if (n < d.N) {
+#pragma unroll 16
+    for (int i = r; i < d.blocks; i += 16) s += d.partial[(long long)i * d.N + n];
+  }
+  sums[r * 17 + c] = s;
+  __syncthreads();
+  if (r == 0 && n < d.N) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sums[i * 17 + c];
+    static_cast<typename T::elem*>(d.db)[n] = from_float<T>(s);
+  }
 }
 
-// ---- joining the splits of a product -------------------------------------------------------------------------------------
-// A block takes 32 groups of eight columns of one tile's rows; 8 lanes share a group's splits.  The order is fixed.
+// 256 / lanes groups of eight columns of one tile's rows a block; `lanes` threads share a group's splits.  The order is
+// fixed.
 template <class T>
-__global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn) {
-  __shared__ float sums[8][32][9];
-  const int c = threadIdx.x & 31, s0 = threadIdx.x >> 5, groups = bn / 8, per_tile = bm * groups / 32;
-  const int tile = blockIdx.x / per_tile, group = (blockIdx.x - tile * per_tile) * 32 + c;
+__global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn, int lanes, unsigned join_blocks, DbArgs db) {
+  __shared__ float sums[256 * 9];
+  if (blockIdx.x >= join_blocks) {
+    db_block<T>(db, blockIdx.x - join_blocks, sums);
+    return;
+  }
+  const int here = 256 / lanes, c = threadIdx.x % here, s0 = threadIdx.x / here, groups = bn / 8, per_tile = bm * groups / here;
+  const int tile = blockIdx.x / per_tile, group = (blockIdx.x - tile * per_tile) * here + c;
   int tm, tn;
   place_of(g, g.whole + tile, tm, tn);
   const long long m = (long long)tm * bm + group / groups;
@@ -157,7 +180,7 @@ __global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn) 
   if (in) {
     const float* p = g.partial + (long long)tile * g.splits * bm * bn + 8 * group;
 #pragma unroll 4
-    for (int s = s0; s < g.splits; s += 8) {
+    for (int s = s0; s < g.splits; s += lanes) {
       float w[8];
       unpack8<Fp32>(load8_raw<Fp32>(p + (long long)s * bm * bn), w);
 #pragma unroll
@@ -165,13 +188,12 @@ __global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn) 
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sums[s0][c][i] = v[0][i];
+  for (int i = 0; i < 8; ++i) sums[threadIdx.x * 9 + i] = v[0][i];
   __syncthreads();
   if (s0 != 0 || !in) return;
+  for (int s = 1; s < lanes; ++s)
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int s = 1; s < 8; ++s) v[0][i] += sums[s][c][i];
+    for (int i = 0; i < 8; ++i) v[0][i] += sums[(s * here + c) * 9 + i];
   DropArgs drop = g.e.drop;
   if (drop.drop) load_offset(drop);
   finish<T, 1>(g.e, drop, {m}, g.M, n, left, v);
@@ -324,14 +346,25 @@ Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
   p.tiles_m = ceil_div(M, p.bm);
   p.tiles_n = ceil_div(N, p.bn);
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
-  // Rounds of one tile a CU are done whole.  The rest would leave CUs idle for a round: it is cut along k until there are
-  // two pieces for every CU (one of the largest block), each of four steps of 32 k at least.
+  // Rounds of one tile a CU are done whole.  The rest would leave CUs idle for a round: it may be cut along k until there are
+  // two pieces for every CU (one of the largest block), of two steps of 32 k at least in float32 and four in 16 bits.
   const int want = p.block == kBlock256x256 ? kCUs : 2 * kCUs;
-  const int others = (int)(tiles % kCUs);
+  const int others = (int)(tiles % kCUs), least = dtype == RNNT_MI355X_FP32 ? 2 : 4;
   p.splits = others == 0 ? 1 : want / others;
-  if (p.splits > steps / 4) p.splits = steps / 4;
-  if (tiles > 16 * kCUs || p.splits < 2) p.splits = 1;
-  p.k_each = ceil_div(ceil_div(K, p.splits), 64) * 64;
+  if (p.splits > steps / least) p.splits = steps / least;
+  if (p.splits < 2) p.splits = 1;
+  if (p.splits > 1) {
+    // What that saves against what joining the pieces costs, in us.  A CU multiplies at 4.3 TFLOP/s in 16 bits (1.1 PFLOP/s of
+    // the card) and at a sixth of it in float32; a block alone on its CU, with nobody to fill its waits, takes a quarter
+    // more and 0.4 a step.  Joining is a launch, and the pieces written and read at 4 TB/s.  Measured, whole against cut:
+    // float32 1200x250x250 24 : 14 us, 6151x1032x520 87 : 69, 6151x520x1032 56 : 66; bfloat16 64x2048x8192 19 : 15, 4096x512x512 10 : 24.
+    double step = 2.0 * p.bm * p.bn * 32 / 4.3e6 * (dtype == RNNT_MI355X_FP32 ? 6 : 1);
+    if (tiles < kCUs) step = 0.4 + 1.25 * step;
+    const double saves = steps * step * (1.0 - 1.0 / p.splits), costs = 5.0 + 2.0 * others * p.splits * p.bm * p.bn * 4 / 4e6;
+    if (saves < costs) p.splits = 1;
+  }
+  const int whole_k = p.block == kBlock32 || dtype != RNNT_MI355X_FP32 ? 64 : 32;  // what the steps of a piece divide
+  p.k_each = ceil_div(ceil_div(K, p.splits), whole_k) * whole_k;
   p.splits = ceil_div(K, p.k_each);
   p.whole = (int)(p.splits == 1 ? tiles : tiles - others);
   p.partial_bytes = (size_t)(tiles - p.whole) * p.splits * p.bm * p.bn * sizeof(float);
@@ -354,7 +387,7 @@ int gemm_of(int product, int block, bool direct, const GemmArgs& g, hipStream_t 
 
 template <class T>
 int run_product(int product, const Plan& p, const void* a, long long a_ld, const void* b, long long b_ld, int M, int N, int K,
-                const Epilogue& e, float* partial, hipStream_t st) {
+                const Epilogue& e, float* partial, hipStream_t st, const DbArgs& db = DbArgs{nullptr, nullptr, 0, 0}) {
   GemmArgs g;
   g.a = a;
   g.b = b;
@@ -372,8 +405,11 @@ int run_product(int product, const Plan& p, const void* a, long long a_ld, const
   g.e = e;
   const int rc = p.block == kBlockRows ? launch_rows<T>(g, st) : gemm_of<T>(product, p.block, p.direct, g, st);
   const int others = p.tiles_m * p.tiles_n - p.whole;
-  if (rc != RNNT_MI355X_OK || others == 0) return rc;
-  k_layer_join<T><<<(unsigned)others * (p.bm * p.bn / 256), 256, 0, st>>>(g, p.bm, p.bn);
+  if (rc != RNNT_MI355X_OK || (others == 0 && !db.db)) return rc;
+  int lanes = p.splits >= 8 ? 8 : p.splits >= 4 ? 4 : 2;
+  if (p.bm * p.bn / 8 < 256 / lanes) lanes = 8;
+  const unsigned join_blocks = (unsigned)others * (unsigned)(p.bm * p.bn / 8 / (256 / lanes));
+  k_layer_join<T><<<join_blocks + (db.db ? (unsigned)ceil_div(db.N, 16) : 0u), 256, 0, st>>>(g, p.bm, p.bn, lanes, join_blocks, db);
   return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
 }
 
@@ -438,22 +474,15 @@ Operand operand(const void* p, long long ld, long long rows, int cols, int dtype
   return o;
 }
 bool direct(const Operand& o, int dtype) { return o.pack || can_go_direct(o.p, o.ld, o.cols, dtype); }
-// The copies of a call, both in one launch; afterwards the operands are their copies.
-int pack(Operand& a, long long a_src_ld, Operand& b, long long b_src_ld, char* ws, hipStream_t st) {
-  PackArgs p[2];
-  unsigned blocks[2] = {0, 0};
-  Operand* o[2] = {&a, &b};
-  for (int i = 0; i < 2; ++i) {
-    p[i] = PackArgs{static_cast<const uint16_t*>(o[i]->p), reinterpret_cast<uint16_t*>(ws + o[i]->at), i ? b_src_ld : a_src_ld, o[i]->ld, o[i]->rows, o[i]->cols};
-    if (!o[i]->pack) continue;
-    const long long n = (o[i]->rows * ((o[i]->cols + 7) / 8) + 255) / 256;
-    if (n > 0x3fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
-    blocks[i] = (unsigned)n;
-    o[i]->p = ws + o[i]->at;
-  }
-  if (blocks[0] + blocks[1] == 0) return RNNT_MI355X_OK;
-  k_layer_pack<<<blocks[0] + blocks[1], 256, 0, st>>>(p[0], p[1], blocks[0]);
-  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+// What copies an operand; afterwards it is its copy.
+int pack_of(Operand& o, long long src_ld, char* ws, PackArgs* p) {
+  *p = PackArgs{static_cast<const uint16_t*>(o.p), reinterpret_cast<uint16_t*>(ws + o.at), src_ld, o.ld, o.rows, o.cols, 0u};
+  if (!o.pack) return RNNT_MI355X_OK;
+  const long long n = (o.rows * ((o.cols + 7) / 8) + 255) / 256;
+  if (n > 0x3fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
+  p->blocks = (unsigned)n;
+  o.p = ws + o.at;
+  return RNNT_MI355X_OK;
 }
 
 constexpr int kOften = 512;  // rows that share the kernel
@@ -480,7 +509,7 @@ struct BackwardPlan {
   bool need_dz;  // else dz is dy
   Operand x, kernel, dz;
   size_t sums_at, partial_at, bytes;
-  int dz_rows, dz_blocks;  // the dz pass: rows of a block, blocks
+  int dz_rows, dz_blocks, dz_across;  // the dz pass: rows of a block, blocks down and across
   Plan dx, dk;
 };
 BackwardPlan plan_backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride) {
@@ -501,8 +530,11 @@ BackwardPlan plan_backward(const rnnt_mi355x_layer* l, const void* dy, long long
   b.x.at = b.dz.bytes;
   b.kernel.at = b.x.at + b.x.bytes;
   b.sums_at = b.kernel.at + b.kernel.bytes;
-  // 2048 blocks, in rows of 8
-  const long long across = ceil_div(l->out, kDzGroups * 8), rows = ((long long)M * across / 2048 + 7) / 8 * 8;
+  // about 8192 blocks, in rows of 8, and at most 2048 partial sums a column
+  b.dz_across = ceil_div(l->out, kDzGroups * 8);
+  const long long most = ((long long)M / 2048 + 7) / 8 * 8;
+  long long rows = ((long long)M * b.dz_across / 8192 + 7) / 8 * 8;
+  if (rows < most) rows = most;
   b.dz_rows = (int)(rows < 8 ? 8 : rows);
   b.dz_blocks = ceil_div(M, b.dz_rows);
   b.partial_at = b.sums_at + align_up((size_t)b.dz_blocks * l->out * sizeof(float));
@@ -522,8 +554,14 @@ int forward(const rnnt_mi355x_layer* l, ForwardPlan f, void* workspace, hipStrea
   e.act = l->act;
   e.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
   char* ws = static_cast<char*>(workspace);
-  const int rc = pack(f.x, l->x_stride, f.kernel, l->kernel_stride, ws, st);
+  PackArgs px, pk;
+  int rc = pack_of(f.x, l->x_stride, ws, &px);
+  if (rc == RNNT_MI355X_OK) rc = pack_of(f.kernel, l->kernel_stride, ws, &pk);
   if (rc != RNNT_MI355X_OK) return rc;
+  if (px.blocks + pk.blocks) {
+    k_layer_pack<<<px.blocks + pk.blocks, 256, 0, st>>>(px, pk);
+    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
+  }
   return run_product<T>(kForward, f.y, f.x.p, f.x.ld, f.kernel.p, f.kernel.ld, (int)l->rows, l->out, l->in, e, reinterpret_cast<float*>(ws + f.partial_at), st);
 }
 
@@ -535,34 +573,43 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
   char* ws = static_cast<char*>(workspace);
   if (b.need_dz) b.dz.p = ws + b.dz.at;
   float *sums = reinterpret_cast<float*>(ws + b.sums_at), *partial = reinterpret_cast<float*>(ws + b.partial_at);
-  if (b.need_dz || dbias) {
-    DzArgs a;
-    a.dy = dy;
-    a.saved = from == kPreActivation ? l->aux : l->y;
-    a.dz = b.need_dz ? ws + b.dz.at : nullptr;
-    a.partial = dbias ? sums : nullptr;
-    a.dy_ld = dy_stride;
-    a.dz_ld = b.dz.ld;
-    a.M = M;
-    a.N = l->out;
-    a.rows = b.dz_rows;
-    a.act = l->act;
-    a.from = from;
-    a.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
-    k_layer_dz<T><<<dim3((unsigned)ceil_div(l->out, kDzGroups * 8), (unsigned)b.dz_blocks), kDzGroups * kDzLanes, 0, st>>>(a);
-    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
-  }
-  if (dbias) {
-    k_layer_db<T><<<(unsigned)ceil_div(l->out, 32), 1024, 0, st>>>(sums, b.dz_blocks, l->out, static_cast<typename T::elem*>(dbias));
-    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
-  }
   if (!dx) b.kernel.pack = false;
   if (!dkernel) b.x.pack = false;
-  int rc = pack(b.x, l->x_stride, b.kernel, l->kernel_stride, ws, st);
-  if (rc == RNNT_MI355X_OK && dx)
-    rc = run_product<T>(kInputGrad, b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), partial, st);
-  if (rc == RNNT_MI355X_OK && dkernel)
-    rc = run_product<T>(kKernelGrad, b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), partial, st);
+  PackArgs px, pk;
+  int rc = pack_of(b.x, l->x_stride, ws, &px);
+  if (rc == RNNT_MI355X_OK) rc = pack_of(b.kernel, l->kernel_stride, ws, &pk);
+  if (rc != RNNT_MI355X_OK) return rc;
+  DzArgs a;
+  a.dy = dy;
+  a.saved = from == kPreActivation ? l->aux : l->y;
+  a.dz = b.need_dz ? ws + b.dz.at : nullptr;
+  a.partial = dbias ? sums : nullptr;
+  a.dy_ld = dy_stride;
+  a.dz_ld = b.dz.ld;
+  a.M = M;
+  a.N = l->out;
+  a.rows = b.dz_rows;
+  a.across = b.dz_across;
+  a.blocks = b.need_dz || dbias ? (unsigned)b.dz_across * (unsigned)b.dz_blocks : 0u;
+  a.act = l->act;
+  a.from = from;
+  a.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
+  if (a.blocks + px.blocks + pk.blocks) {
+    k_layer_dz<T><<<a.blocks + px.blocks + pk.blocks, kDzGroups * kDzLanes, 0, st>>>(a, px, pk);
+    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
+  }
+  DbArgs db{sums, dbias, b.dz_blocks, l->out};
+  if (dx) {
+    rc = run_product<T>(kInputGrad, b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), partial, st,
+                        dkernel ? DbArgs{nullptr, nullptr, 0, 0} : db);
+    if (rc != RNNT_MI355X_OK) return rc;
+  }
+  if (dkernel) return run_product<T>(kKernelGrad, b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), partial, st, db);
+  if (!dx && dbias) {
+    GemmArgs none{};
+    k_layer_join<T><<<(unsigned)ceil_div(l->out, 16), 256, 0, st>>>(none, 8, 8, 8, 0u, db);
+    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
+  }
   return rc;
 }
 

@@ -11,14 +11,14 @@ import ctypes
 import torch
 
 from . import _lib
-from ._operator import check, drop16, dtype_code, need_gpu, on_device, seed_offset, stream
+from ._operator import DTYPE_CODE, check, drop16, dtype_code, need_gpu, on_device, seed_offset, stream
 
 ACTIVATIONS = {"linear": 0, "tanh": 1, "relu": 2, "gelu": 3, "silu": 4}
 _AUX_TYPE = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 
 
 def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    return None if t is None else t.data_ptr()
 
 
 def _as_rows(t):
@@ -33,35 +33,38 @@ def _as_rows(t):
     return t, max(t.stride(0), n) if t.shape[0] > 1 else n
 
 
-def _layer(x, x_stride, kernel, kernel_stride, code, act, drop, seed, offset, offset_t):
-    return _lib.Layer(x=x.data_ptr(), kernel=kernel.data_ptr(), x_stride=x_stride, kernel_stride=kernel_stride, rows=x.shape[0],
-                      n_in=kernel.shape[0], n_out=kernel.shape[1], dtype=code, act=act, drop16=drop, seed=seed, offset=offset,
-                      offset_dev=_ptr(offset_t))
+def _layer(x, x_stride, kernel, kernel_stride, bias, residual, residual_stride, y, aux, act, drop, seed, offset, offset_t):
+    n_in, n_out = kernel.shape
+    # positional: the order of rnnt_mi355x_layer
+    return _lib.Layer(x.data_ptr(), kernel.data_ptr(), _ptr(bias), _ptr(residual), _ptr(y), _ptr(aux), x_stride, kernel_stride, residual_stride,
+                      x.shape[0], n_in, n_out, DTYPE_CODE[x.dtype], act, drop, seed, offset, _ptr(offset_t))
 
 
 def _forward(x, kernel, bias, residual, act, drop, seed, offset, offset_t, want_aux):
     """(y, aux or None)"""
-    shape = x.shape[:-1] + (kernel.shape[1],)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    aux = torch.empty(shape, dtype=_AUX_TYPE[x.dtype], device=x.device) if want_aux else None
+    dev, shape = x.device, (*x.shape[:-1], kernel.shape[1])
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    aux = torch.empty(shape, dtype=_AUX_TYPE[x.dtype], device=dev) if want_aux else None
     if y.numel() == 0:
         return y, aux
     x, x_stride = _as_rows(x)
     kernel, kernel_stride = _as_rows(kernel)
-    layer = _layer(x, x_stride, kernel, kernel_stride, dtype_code("dense", x), act, drop, seed, offset, offset_t)
-    if bias is not None:
+    residual_stride, ws_p = 0, None
+    if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-        layer.bias = bias.data_ptr()
     if residual is not None:
-        residual, layer.residual_stride = _as_rows(residual)
-        layer.residual = residual.data_ptr()
-    layer.y, layer.aux = y.data_ptr(), _ptr(aux)
+        residual, residual_stride = _as_rows(residual)
+    layer = ctypes.byref(_layer(x, x_stride, kernel, kernel_stride, bias, residual, residual_stride, y, aux, act, drop, seed, offset, offset_t))
     L = _lib.lib()
-    with on_device(x.device):
+    with on_device(dev):
         n = ctypes.c_size_t(0)
-        check(L.rnnt_mi355x_layer_workspace_bytes(ctypes.byref(layer), None, 0, ctypes.byref(n), None), "rnnt_mi355x_layer_workspace_bytes")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device) if n.value else None
-        check(L.rnnt_mi355x_layer_forward(ctypes.byref(layer), _ptr(ws), stream(x.device)), "rnnt_mi355x_layer_forward")
+        rc = L.rnnt_mi355x_layer_workspace_bytes(layer, None, 0, ctypes.byref(n), None)
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+            ws_p = ws.data_ptr()
+        rc = rc or L.rnnt_mi355x_layer_forward(layer, ws_p, stream(dev))
+    if rc:
+        check(rc, "rnnt_mi355x_layer_forward")
     return y, aux
 
 
@@ -94,16 +97,16 @@ class _LayerFn(torch.autograd.Function):
         x, x_stride = _as_rows(x)
         kernel, kernel_stride = _as_rows(kernel)
         dy, dy_stride = _as_rows(dy)
-        layer = _layer(x, x_stride, kernel, kernel_stride, dtype_code("dense", x), *ctx.args, offset_t)
-        layer.y, layer.aux = _ptr(y), _ptr(aux)
+        dev, dy_p = x.device, dy.data_ptr()
+        layer = ctypes.byref(_layer(x, x_stride, kernel, kernel_stride, None, None, 0, y, aux, *ctx.args, offset_t))
         L = _lib.lib()
-        with on_device(x.device):
+        with on_device(dev):
             n = ctypes.c_size_t(0)
-            check(L.rnnt_mi355x_layer_workspace_bytes(ctypes.byref(layer), dy.data_ptr(), dy_stride, None, ctypes.byref(n)),
-                  "rnnt_mi355x_layer_workspace_bytes")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
-            check(L.rnnt_mi355x_layer_backward(ctypes.byref(layer), dy.data_ptr(), dy_stride, _ptr(dx), _ptr(dk), _ptr(db), ws.data_ptr(),
-                                               stream(x.device)), "rnnt_mi355x_layer_backward")
+            rc = L.rnnt_mi355x_layer_workspace_bytes(layer, dy_p, dy_stride, None, ctypes.byref(n))
+            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+            rc = rc or L.rnnt_mi355x_layer_backward(layer, dy_p, dy_stride, _ptr(dx), _ptr(dk), _ptr(db), ws.data_ptr(), stream(dev))
+        if rc:
+            check(rc, "rnnt_mi355x_layer_backward")
         return (dx, dk, db, d_residual) + (None,) * 5
 
 

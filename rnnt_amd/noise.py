@@ -14,17 +14,20 @@ from ._operator import DTYPE_CODE, check, drop16, dtype_code, need_gpu, on_devic
 
 
 def _apply(x, drop, seed, offset, offset_t):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     cols = stride = x.shape[-1]
-    if not x.is_contiguous():
+    if x.is_contiguous():
+        y = torch.empty_like(x)
+    else:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         # rows of a matrix may be any distance apart; anything else is made dense
         if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
             stride = x.stride(0)
         else:
             x = x.contiguous()
-    with on_device(x.device):
+    dev = x.device
+    with on_device(dev):
         rc = _lib.lib().rnnt_mi355x_dropout(x.data_ptr(), stride, y.data_ptr(), x.numel() // cols, cols, DTYPE_CODE[x.dtype], drop, seed, offset,
-                                            None if offset_t is None else offset_t.data_ptr(), stream(x.device))
+                                            None if offset_t is None else offset_t.data_ptr(), stream(dev))
     if rc:
         check(rc, "rnnt_mi355x_dropout")
     return y
