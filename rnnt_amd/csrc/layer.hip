@@ -160,29 +160,31 @@ __device__ __forceinline__ void db_block(const DbArgs& d, unsigned block, float*
   }
 }
 
-// 256 / lanes groups of eight columns of one tile's rows a block; `lanes` threads share a group's splits.  The order is
-// fixed.
+// The cut tiles of a product: 256 / lanes groups of eight columns of one tile's rows a block; `lanes` threads share a group's
+// splits.  The order is fixed.
+struct JoinArgs {
+  GemmArgs g;
+  int bm, bn, lanes;
+  unsigned blocks;
+};
 template <class T>
-__global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn, int lanes, unsigned join_blocks, DbArgs db) {
-  __shared__ float sums[256 * 9];
-  if (blockIdx.x >= join_blocks) {
-    db_block<T>(db, blockIdx.x - join_blocks, sums);
-    return;
-  }
-  const int here = 256 / lanes, c = threadIdx.x % here, s0 = threadIdx.x / here, groups = bn / 8, per_tile = bm * groups / here;
-  const int tile = blockIdx.x / per_tile, group = (blockIdx.x - tile * per_tile) * here + c;
+__device__ __forceinline__ void join_block(const JoinArgs& j, unsigned block, float* sums) {
+  const GemmArgs& g = j.g;
+  const int here = 256 / j.lanes, c = threadIdx.x % here, s0 = threadIdx.x / here, groups = j.bn / 8, per_tile = j.bm * groups / here;
+  const int tile = block / per_tile, group = (block - tile * per_tile) * here + c;
   int tm, tn;
   place_of(g, g.whole + tile, tm, tn);
-  const long long m = (long long)tm * bm + group / groups;
-  const int n = tn * bn + 8 * (group % groups), left = g.N - n;
+  const long long m = (long long)tm * j.bm + group / groups;
+  const int n = tn * j.bn + 8 * (group % groups), left = g.N - n;
   const bool in = m < g.M && left > 0;
   float v[1][8] = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
   if (in) {
-    const float* p = g.partial + (long long)tile * g.splits * bm * bn + 8 * group;
+    const long long piece = (long long)j.bm * j.bn;
+    const float* p = g.partial + tile * g.splits * piece + 8 * group;
 #pragma unroll 4
-    for (int s = s0; s < g.splits; s += lanes) {
+    for (int s = s0; s < g.splits; s += j.lanes) {
       float w[8];
-      unpack8<Fp32>(load8_raw<Fp32>(p + (long long)s * bm * bn), w);
+      unpack8<Fp32>(load8_raw<Fp32>(p + s * piece), w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[0][i] += w[i];
     }
@@ -191,12 +193,21 @@ __global__ __launch_bounds__(256) void k_layer_join(GemmArgs g, int bm, int bn, 
   for (int i = 0; i < 8; ++i) sums[threadIdx.x * 9 + i] = v[0][i];
   __syncthreads();
   if (s0 != 0 || !in) return;
-  for (int s = 1; s < lanes; ++s)
+  for (int s = 1; s < j.lanes; ++s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[0][i] += sums[(s * here + c) * 9 + i];
   DropArgs drop = g.e.drop;
   if (drop.drop) load_offset(drop);
   finish<T, 1>(g.e, drop, {m}, g.M, n, left, v);
+}
+// What is left after the products of a call, in one launch.
+template <class T>
+__global__ __launch_bounds__(256) void k_layer_join(JoinArgs a, JoinArgs b, DbArgs db) {
+  __shared__ float sums[256 * 9];
+  const unsigned id = blockIdx.x;
+  if (id < a.blocks) join_block<T>(a, id, sums);
+  else if (id < a.blocks + b.blocks) join_block<T>(b, id - a.blocks, sums);
+  else db_block<T>(db, id - a.blocks - b.blocks, sums);
 }
 
 // ---- a decoder's few rows ------------------------------------------------------------------------------------------------
@@ -332,6 +343,23 @@ Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
     p.partial_bytes = p.whole ? 0 : (size_t)p.tiles_n * p.splits * p.bm * p.bn * sizeof(float);
     return p;
   }
+  if (product != kKernelGrad && M <= 64 && ceil_div(N, 64) >= 32) {
+    // Few rows of a wide layer: a block for every CU at most, in which four groups share k; pieces of k only where blocks are
+    // fewer, of 1024 or more.  Against blocks of one group and more pieces: 64 x 2048 x 8192 bfloat16 14.7 us (16.1), float32
+    // 27 (33), 64 x 4096 x 16384 float32 82 (124), 32 x 512 x 4096 float32 9.0 (11.5); with fewer columns the pieces win.
+    p.block = M <= 32 ? kBlock32Groups : kBlock64Groups;
+    p.bm = M <= 32 ? 32 : 64;
+    p.bn = 64;
+    p.tiles_m = 1;
+    p.tiles_n = ceil_div(N, 64);
+    p.splits = kCUs / p.tiles_n < K / 1024 ? kCUs / p.tiles_n : K / 1024;
+    if (p.splits < 1) p.splits = 1;
+    p.k_each = ceil_div(ceil_div(K, p.splits), 64) * 64;
+    p.splits = ceil_div(K, p.k_each);
+    p.whole = p.splits == 1 ? p.tiles_n : 0;
+    p.partial_bytes = (size_t)(p.tiles_n - p.whole) * p.splits * p.bm * p.bn * sizeof(float);
+    return p;
+  }
   if (product != kKernelGrad && M <= 32) {
     p.block = kBlock32;
     p.bm = 32;
@@ -386,8 +414,13 @@ int gemm_of(int product, int block, bool direct, const GemmArgs& g, hipStream_t 
 }
 
 template <class T>
-int run_product(int product, const Plan& p, const void* a, long long a_ld, const void* b, long long b_ld, int M, int N, int K,
-                const Epilogue& e, float* partial, hipStream_t st, const DbArgs& db = DbArgs{nullptr, nullptr, 0, 0}) {
+int grads_of(bool direct, const GemmArgs& dx, const GemmArgs& dk, hipStream_t st) {
+  if constexpr (T::code == RNNT_MI355X_FP32) return layer_grads_fp32(direct, &dx, &dk, st);
+  else if constexpr (T::code == RNNT_MI355X_BF16) return layer_grads_bf16(direct, &dx, &dk, st);
+  else return layer_grads_fp16(direct, &dx, &dk, st);
+}
+
+GemmArgs product_args(const Plan& p, const void* a, long long a_ld, const void* b, long long b_ld, int M, int N, int K, const Epilogue& e, void* partial) {
   GemmArgs g;
   g.a = a;
   g.b = b;
@@ -401,16 +434,34 @@ int run_product(int product, const Plan& p, const void* a, long long a_ld, const
   g.whole = p.whole;
   g.splits = p.splits;
   g.k_each = p.k_each;
-  g.partial = partial;
+  g.partial = static_cast<float*>(partial);
   g.e = e;
-  const int rc = p.block == kBlockRows ? launch_rows<T>(g, st) : gemm_of<T>(product, p.block, p.direct, g, st);
-  const int others = p.tiles_m * p.tiles_n - p.whole;
-  if (rc != RNNT_MI355X_OK || (others == 0 && !db.db)) return rc;
-  int lanes = p.splits >= 8 ? 8 : p.splits >= 4 ? 4 : 2;
-  if (p.bm * p.bn / 8 < 256 / lanes) lanes = 8;
-  const unsigned join_blocks = (unsigned)others * (unsigned)(p.bm * p.bn / 8 / (256 / lanes));
-  k_layer_join<T><<<join_blocks + (db.db ? (unsigned)ceil_div(db.N, 16) : 0u), 256, 0, st>>>(g, p.bm, p.bn, lanes, join_blocks, db);
+  return g;
+}
+
+JoinArgs join_args(const Plan& p, const GemmArgs& g) {
+  JoinArgs j{g, p.bm, p.bn, p.splits >= 8 ? 8 : p.splits >= 4 ? 4 : 2, 0u};
+  if (p.bm * p.bn / 8 < 256 / j.lanes) j.lanes = 8;
+  j.blocks = (unsigned)(p.tiles_m * p.tiles_n - p.whole) * (unsigned)(p.bm * p.bn / 8 / (256 / j.lanes));
+  return j;
+}
+JoinArgs no_join() {
+  JoinArgs j{};
+  j.lanes = 1;
+  return j;
+}
+
+template <class T>
+int run_join(const JoinArgs& a, const JoinArgs& b, const DbArgs& db, hipStream_t st) {
+  const unsigned blocks = a.blocks + b.blocks + (db.db ? (unsigned)ceil_div(db.N, 16) : 0u);
+  if (blocks == 0) return RNNT_MI355X_OK;
+  k_layer_join<T><<<blocks, 256, 0, st>>>(a, b, db);
   return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+}
+
+template <class T>
+int run_product(int product, const Plan& p, const GemmArgs& g, hipStream_t st) {
+  return p.block == kBlockRows ? launch_rows<T>(g, st) : gemm_of<T>(product, p.block, p.direct, g, st);
 }
 
 Epilogue plain_output(void* out, long long ld) {
@@ -540,7 +591,7 @@ BackwardPlan plan_backward(const rnnt_mi355x_layer* l, const void* dy, long long
   b.partial_at = b.sums_at + align_up((size_t)b.dz_blocks * l->out * sizeof(float));
   b.dx = plan_product(kInputGrad, dtype, M, l->in, l->out, direct(b.dz, dtype) && direct(b.kernel, dtype));
   b.dk = plan_product(kKernelGrad, dtype, l->in, l->out, M, direct(b.dz, dtype) && direct(b.x, dtype));
-  b.bytes = b.partial_at + (b.dx.partial_bytes > b.dk.partial_bytes ? b.dx.partial_bytes : b.dk.partial_bytes);
+  b.bytes = b.partial_at + align_up(b.dx.partial_bytes) + b.dk.partial_bytes;
   return b;
 }
 
@@ -562,7 +613,9 @@ int forward(const rnnt_mi355x_layer* l, ForwardPlan f, void* workspace, hipStrea
     k_layer_pack<<<px.blocks + pk.blocks, 256, 0, st>>>(px, pk);
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
   }
-  return run_product<T>(kForward, f.y, f.x.p, f.x.ld, f.kernel.p, f.kernel.ld, (int)l->rows, l->out, l->in, e, reinterpret_cast<float*>(ws + f.partial_at), st);
+  const GemmArgs g = product_args(f.y, f.x.p, f.x.ld, f.kernel.p, f.kernel.ld, (int)l->rows, l->out, l->in, e, ws + f.partial_at);
+  rc = run_product<T>(kForward, f.y, g, st);
+  return rc == RNNT_MI355X_OK ? run_join<T>(join_args(f.y, g), no_join(), DbArgs{}, st) : rc;
 }
 
 template <class T>
@@ -572,7 +625,7 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
   const int M = (int)l->rows;
   char* ws = static_cast<char*>(workspace);
   if (b.need_dz) b.dz.p = ws + b.dz.at;
-  float *sums = reinterpret_cast<float*>(ws + b.sums_at), *partial = reinterpret_cast<float*>(ws + b.partial_at);
+  float* sums = reinterpret_cast<float*>(ws + b.sums_at);
   if (!dx) b.kernel.pack = false;
   if (!dkernel) b.x.pack = false;
   PackArgs px, pk;
@@ -598,18 +651,16 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
     k_layer_dz<T><<<a.blocks + px.blocks + pk.blocks, kDzGroups * kDzLanes, 0, st>>>(a, px, pk);
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
   }
-  DbArgs db{sums, dbias, b.dz_blocks, l->out};
-  if (dx) {
-    rc = run_product<T>(kInputGrad, b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), partial, st,
-                        dkernel ? DbArgs{nullptr, nullptr, 0, 0} : db);
-    if (rc != RNNT_MI355X_OK) return rc;
+  const GemmArgs gx = product_args(b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), ws + b.partial_at);
+  const GemmArgs gk = product_args(b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), ws + b.partial_at + align_up(b.dx.partial_bytes));
+  if (dx && dkernel && b.dx.block == kBlock128x128 && b.dk.block == kBlock128x128 && b.dx.direct == b.dk.direct) {
+    rc = grads_of<T>(b.dx.direct, gx, gk, st);
+  } else {
+    if (dx) rc = run_product<T>(kInputGrad, b.dx, gx, st);
+    if (rc == RNNT_MI355X_OK && dkernel) rc = run_product<T>(kKernelGrad, b.dk, gk, st);
   }
-  if (dkernel) return run_product<T>(kKernelGrad, b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), partial, st, db);
-  if (!dx && dbias) {
-    GemmArgs none{};
-    k_layer_join<T><<<(unsigned)ceil_div(l->out, 16), 256, 0, st>>>(none, 8, 8, 8, 0u, db);
-    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
-  }
+  if (rc == RNNT_MI355X_OK)
+    rc = run_join<T>(dx ? join_args(b.dx, gx) : no_join(), dkernel ? join_args(b.dk, gk) : no_join(), DbArgs{sums, dbias, b.dz_blocks, l->out}, st);
   return rc;
 }
 

@@ -228,6 +228,9 @@ struct Tile {
   static constexpr int kPlaneBytes = R * BK * 2, kBytes = kPlaneBytes * kPlanes<T>;
   static_assert(kPieces % THREADS == 0 && (!KS || R >= 64) && (BK == 32 || BK == 64), "tile shape");
 
+  static_assert((THREADS & (THREADS - 1)) == 0, "");
+  static __device__ __forceinline__ int tid() { return threadIdx.x & (THREADS - 1); }  // of the wavefronts that share this tile
+
   // place p holds row p / kRow and piece (p % kRow) ^ permute(row).  64 banks serve 256 bytes a cycle: k-fast reads take one
   // piece of 16 rows together, k-slow reads 64 bytes of 4 consecutive k.
   static __device__ __forceinline__ int permute(int row) {
@@ -239,7 +242,7 @@ struct Tile {
   static __device__ __forceinline__ void load(Raw8<T> (&raw)[kEach], const E* base, long long ld, int r0, int r_end, int k0, int k_end) {
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int p = j * THREADS + threadIdx.x, row = p / kRow, piece = (p % kRow) ^ permute(row);
+      const int p = j * THREADS + tid(), row = p / kRow, piece = (p % kRow) ^ permute(row);
       // outer: the strided index, inner: the contiguous one
       const int outer = KS ? k0 + row : r0 + row, inner = KS ? r0 + 8 * piece : k0 + 8 * piece;
       const int outer_end = KS ? k_end : r_end, inner_end = KS ? r_end : k_end;
@@ -262,7 +265,7 @@ struct Tile {
   static __device__ __forceinline__ void store(const Raw8<T> (&raw)[kEach], char* lds) {
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int p = j * THREADS + threadIdx.x;
+      const int p = j * THREADS + tid();
       if constexpr (kPlanes<T> == 3) {
         float v[8];
         u4 q[3];
@@ -293,14 +296,14 @@ struct Tile {
       left = k_end - k0;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
-        const int p = j * THREADS + threadIdx.x, row = p / kRow, piece = (p % kRow) ^ permute(row);
+        const int p = j * THREADS + tid(), row = p / kRow, piece = (p % kRow) ^ permute(row);
         k[j] = KS ? row : 8 * piece;
         offset[j] = (KS ? r0 + 8 * piece < r_end : r0 + row < r_end) ? (row * (int)ld + 8 * piece) * 2 : 0x7ffffff0;
       }
     }
     __device__ __forceinline__ void next(char* lds) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass has no type for the buffer descriptor and would drop the kernel's launch stub
-      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      const int wave = __builtin_amdgcn_readfirstlane(tid() >> 6);
       auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(corner), 0, (int)(span < 0 ? 0 : span < 0x7ffffff0ll ? span : 0x7ffffff0ll), 0x00020000);
 #pragma unroll
       for (int j = 0; j < kEach; ++j)
@@ -395,9 +398,8 @@ struct Work {
   float* partial;  // null: the tile is whole
 };
 template <int BM, int BN>
-__device__ __forceinline__ Work work_of(const GemmArgs& g) {
+__device__ __forceinline__ Work work_of(const GemmArgs& g, int id) {
   Work w;
-  const int id = blockIdx.x;
   if (id < g.whole) {
     place_of(g, dealt(id, g.whole), w.tm, w.tn);
     w.k0 = 0;
@@ -412,6 +414,50 @@ __device__ __forceinline__ Work work_of(const GemmArgs& g) {
     w.partial = g.partial + ((long long)tile * g.splits + split) * (BM * BN);
   }
   return w;
+}
+
+// Steps of BK that each of the groups takes.
+template <int BK, int GROUPS>
+__device__ __forceinline__ int steps_of(const Work& w) {
+  return (w.k1 - w.k0 + GROUPS * BK - 1) / (GROUPS * BK);
+}
+// The groups' sums join in the first group's accumulators, in the groups' order.  place[o]: kSums bytes of LDS for group o > 0,
+// not in use for anything else.
+template <int IM, int IN, int THREADS>
+constexpr int kSums = IM * IN * 16 * THREADS * 4;
+template <int IM, int IN, int GROUPS, int THREADS>
+__device__ __forceinline__ void join_groups(f16v (&acc)[IM][IN], char* const (&place)[GROUPS], int group) {
+  const int tid = threadIdx.x & (THREADS - 1);
+#pragma unroll
+  for (int o = 1; o < GROUPS; ++o) {
+    if (group != o) continue;
+    f4* mine = reinterpret_cast<f4*>(place[o]);
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+      for (int j = 0; j < IN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f16v& r = acc[i][j];
+          mine[((i * IN + j) * 4 + q) * THREADS + tid] = f4{r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]};
+        }
+  }
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int o = 1; o < GROUPS; ++o) {
+    const f4* other = reinterpret_cast<const f4*>(place[o]);
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+      for (int j = 0; j < IN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4 v = other[((i * IN + j) * 4 + q) * THREADS + tid];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[i][j][4 * q + x] += v[x];
+        }
+  }
 }
 
 // A wavefront's 32 IM x 32 IN block of the result, through LDS into rows: eight consecutive n a lane, 32 rows by (up to) 64
@@ -499,18 +545,29 @@ __device__ __forceinline__ void write_result(const GemmArgs& g, f16v (&acc)[IM][
 
 // Any alignment and type: tiles come through registers, where float32 is split.  WM x WN of the result per wavefront.
 // The next tile is on its way while one is multiplied, and other blocks of the CU multiply while this one splits and stores.
-template <class T, bool A_KS, bool B_KS, int BM, int BN, int BK, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 1) void k_layer_gemm(GemmArgs g) {
+// GROUPS > 1: as many groups of wavefronts share k, each with a tile of its own (few rows: a block then reads its part of W with
+// all its wavefronts and joins their sums in LDS, where pieces of k on several blocks would go through memory).
+template <class T, int BM, int BN, int BK, int WM, int WN, int GROUPS>
+constexpr int registers_lds() {
+  constexpr int kThreads = (BM / WM) * (BN / WN) * 64, kStage = (BM + BN) * BK * 2 * kPlanes<T>, kOut = (kThreads / 64) * kWayOut<WN / 32>;
+  constexpr int kOwn = GROUPS == 1 ? kOut : kSums<WM / 32, WN / 32, kThreads>;
+  return GROUPS * (kStage > kOwn ? kStage : kOwn);
+}
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int BK, int WM, int WN, int GROUPS>  // 1 or 4
+__device__ __forceinline__ void gemm_registers(const GemmArgs& g, int id, char* lds) {
   constexpr int kThreads = (BM / WM) * (BN / WN) * 64, IM = WM / 32, IN = WN / 32;
   using TA = Tile<T, A_KS, BM, BK, kThreads>;
   using TB = Tile<T, B_KS, BN, BK, kThreads>;
   using E = typename T::elem;
-  constexpr int kStage = TA::kBytes + TB::kBytes, kOut = (kThreads / 64) * kWayOut<IN>;
-  __shared__ __attribute__((aligned(16))) char buf[kStage > kOut ? kStage : kOut];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int kBuffer = registers_lds<T, BM, BN, BK, WM, WN, GROUPS>();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x & (kThreads - 1)) >> 6);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  char* buf = lds + group * (kBuffer / GROUPS);
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-  const Work w = work_of<BM, BN>(g);
-  const int m0 = w.tm * BM, n0 = w.tn * BN, k0 = w.k0, k1 = w.k1;
+  const Work w = work_of<BM, BN>(g, id);
+  const int m0 = w.tm * BM, n0 = w.tn * BN, steps = steps_of<BK, GROUPS>(w);
+  int k0 = w.k0 + group * steps * BK;
+  const int k1 = min(w.k1, k0 + steps * BK);
   const E *a = static_cast<const E*>(g.a), *b = static_cast<const E*>(g.b);
 
   f16v acc[IM][IN];
@@ -553,14 +610,20 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 1) void
     }
   };
   fetch(k0);
-  for (int k = k0; k < k1; k += BK) {
+  for (int left = steps; left > 0; --left) {
     put(buf);
     __syncthreads();
-    if (k + BK < k1) fetch(k + BK);
+    k0 += BK;
+    if (left > 1) fetch(k0);  // past k1: zeros
     multiply(buf);
     __syncthreads();
   }
-  write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, buf + wave * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
+  if constexpr (GROUPS > 1) {
+    char* const place[GROUPS] = {lds, lds + kBuffer / GROUPS, lds + kBuffer / GROUPS * 2, lds + kBuffer / GROUPS * 3};
+    join_groups<IM, IN, GROUPS, kThreads>(acc, place, group);
+    if (group != 0) return;
+  }
+  write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, lds + wave * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
 }
 
 // Operands of 16-bit types whose rows are whole 16-byte pieces on 16-byte boundaries (with zeros in the last piece behind the
@@ -569,20 +632,21 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 1) void
 // the oldest one any more, whose buffer is then filled again.
 // While step t is multiplied, tiles t+2 and t+3 are on their way and t+1 is there, so that its first fragments are read before
 // the barrier that ends the step.
-template <class T, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm_ring(GemmArgs g) {
+// GROUPS, 1 or 4: as above.
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int GROUPS>
+__device__ __forceinline__ void gemm_ring(const GemmArgs& g, int id, char* lds0, char* lds1, char* lds2, char* lds3) {
   constexpr int kThreads = (BM / WM) * (BN / WN) * 64, IM = WM / 32, IN = WN / 32, BK = 32;
   using TA = Tile<T, A_KS, BM, BK, kThreads>;
   using TB = Tile<T, B_KS, BN, BK, kThreads>;
   using E = typename T::elem;
   constexpr int kStage = TA::kBytes + TB::kBytes, kLoads = TA::kEach + TB::kEach, kHalf = kThreads / 128;
   static_assert(kHalf * kWayOut<IN> <= kStage, "half of the wavefronts have their way out in the first buffer, half in the second");
-  // objects of their own, so that the compiler sees that a tile on its way does not touch the ones being read
-  __shared__ __attribute__((aligned(16))) char buf0[kStage], buf1[kStage], buf2[kStage], buf3[kStage];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x & (kThreads - 1)) >> 6);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  char *buf0 = lds0 + group * kStage, *buf1 = lds1 + group * kStage, *buf2 = lds2 + group * kStage, *buf3 = lds3 + group * kStage;
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-  const Work w = work_of<BM, BN>(g);
-  const int m0 = w.tm * BM, n0 = w.tn * BN, k0 = w.k0, k1 = w.k1;
+  const Work w = work_of<BM, BN>(g, id);
+  const int m0 = w.tm * BM, n0 = w.tn * BN, steps = steps_of<BK, GROUPS>(w), k0 = w.k0 + group * steps * BK, k1 = min(w.k1, k0 + steps * BK);
   typename TA::Source sa;
   typename TB::Source sb;
   sa.init(static_cast<const E*>(g.a), g.a_ld, m0, g.M, k0, k1);
@@ -625,7 +689,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm_ring(
   fetch(buf2);
   landed<kLoads>();
   read(0, buf0, 0);
-  for (int left = (k1 - k0 + BK - 1) / BK;;) {
+  for (int left = steps;;) {
     step(buf0, buf1, buf3);
     if (--left == 0) break;
     step(buf1, buf2, buf0);
@@ -636,7 +700,46 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_layer_gemm_ring(
     if (--left == 0) break;
   }
   __syncthreads();  // also waits for the tiles past the end, which are still on their way
+  if constexpr (GROUPS > 1) {
+    static_assert(kSums<IM, IN, kThreads> <= kStage * GROUPS && kThreads / 64 * kWayOut<IN> <= kStage * GROUPS, "");
+    char* const place[GROUPS] = {lds0, lds1, lds2, lds3};
+    join_groups<IM, IN, GROUPS, kThreads>(acc, place, group);
+    if (group != 0) return;
+    write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, lds0 + wave * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
+    return;
+  }
   write_result<T, A_KS, B_KS, BN, IM, IN>(g, acc, (wave < kHalf ? buf0 : buf1) + (wave % kHalf) * kWayOut<IN>, m0 + wm, n0 + wn, w, wm, wn);
+}
+
+// One product.
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int BK, int WM, int WN, int GROUPS>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64 * GROUPS, BM == 128 ? 3 : 1) void k_layer_gemm(GemmArgs g) {
+  __shared__ __attribute__((aligned(16))) char lds[registers_lds<T, BM, BN, BK, WM, WN, GROUPS>()];
+  gemm_registers<T, A_KS, B_KS, BM, BN, BK, WM, WN, GROUPS>(g, blockIdx.x, lds);
+}
+// LDS buffers are objects of their own, so that the compiler sees that a tile on its way does not touch the ones being read.
+template <class T, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int GROUPS>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64 * GROUPS) void k_layer_gemm_ring(GemmArgs g) {
+  constexpr int kStage = (BM + BN) * 32 * 2 * GROUPS;
+  __shared__ __attribute__((aligned(16))) char lds0[kStage], lds1[kStage], lds2[kStage], lds3[kStage];
+  gemm_ring<T, A_KS, B_KS, BM, BN, WM, WN, GROUPS>(g, blockIdx.x, lds0, lds1, lds2, lds3);
+}
+
+// Both gradients of a layer in one launch, 128 x 128 blocks: they need nothing of one another, and the blocks of the second
+// fill what the last round of the first leaves idle.
+template <class T>
+__global__ __launch_bounds__(256, 3) void k_layer_grads(GemmArgs dx, GemmArgs dk, unsigned dx_blocks) {
+  __shared__ __attribute__((aligned(16))) char lds[registers_lds<T, 128, 128, 32 * (kPlanes<T> == 1 ? 2 : 1), 64, 64, 1>()];
+  constexpr int BK = kPlanes<T> == 1 ? 64 : 32;
+  if (blockIdx.x < dx_blocks) gemm_registers<T, false, false, 128, 128, BK, 64, 64, 1>(dx, blockIdx.x, lds);
+  else gemm_registers<T, true, true, 128, 128, BK, 64, 64, 1>(dk, blockIdx.x - dx_blocks, lds);
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_layer_grads_ring(GemmArgs dx, GemmArgs dk, unsigned dx_blocks) {
+  constexpr int kStage = (128 + 128) * 32 * 2;
+  __shared__ __attribute__((aligned(16))) char lds0[kStage], lds1[kStage], lds2[kStage], lds3[kStage];
+  if (blockIdx.x < dx_blocks) gemm_ring<T, false, false, 128, 128, 64, 64, 1>(dx, blockIdx.x, lds0, lds1, lds2, lds3);
+  else gemm_ring<T, true, true, 128, 128, 64, 64, 1>(dk, blockIdx.x - dx_blocks, lds0, lds1, lds2, lds3);
 }
 
 }  // namespace

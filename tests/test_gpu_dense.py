@@ -91,7 +91,8 @@ def check_layer(M, K, N, dtype, act="linear", bias=True, residual=False, rate=0.
 
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (8, 250, 62), (31, 33, 40), (32, 64, 128), (33, 64, 72), (64, 520, 136), (65, 129, 66),
           (100, 1000, 65), (130, 96, 130), (257, 72, 264), (300, 515, 103), (129, 2056, 136), (1000, 40, 250),
-          (600, 515, 1030), (513, 77, 33), (520, 64, 65), (777, 1003, 130)]
+          (600, 515, 1030), (513, 77, 33), (520, 64, 65), (777, 1003, 130),
+          (24, 2100, 2100), (64, 1500, 2056), (33, 100, 4096), (20, 1032, 2048)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
