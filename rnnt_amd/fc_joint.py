@@ -15,16 +15,20 @@ gradient gives both reduced gradients.  With a single layer the joint is an
 additive one and goes straight to the fused additive-joint loss, so not even
 [B,T,U+1,V] is formed.  The following layers multiply a [B*T*(U+1), hidden]
 matrix by a small kernel: up to 128 x 128 they run on hand-written tall-skinny
-MFMA kernels (weights resident in LDS), beyond that on the library GEMM.  Dropout (training-time noise, keras_model.py:102-103)
-is not part of these functions.
+MFMA kernels (weights resident in LDS), beyond that on the library GEMM.  With dropout (training-time noise,
+keras_model.py:102-103) the hidden layers run as ``dense``, which draws the mask
+in its epilogue and again in its backward pass, at any width.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
+from ._operator import drop16
 from .lambdas import REFERENCE_BLANK_LABEL, SHIFT, rnnt_lambda_func
+from .layer import dense
 from .loss import _ptr, _stream_ptr, rnnt_loss
+from .noise import dropout as _dropout
 
 
 def concatenate_lambda(args):
@@ -128,15 +132,20 @@ def joint_dense(x, kernel, bias, activation="linear"):
                           1 if activation == "tanh" else 0)
 
 
-def fc_joint(y_trans, y_pred, weights):
+def fc_joint(y_trans, y_pred, weights, dropout=0.0, seed=0, offset=0):
     """concatenate_lambda + get_fc without the tiled tensor.
 
     weights: [(kernel[in,out], bias[out]), ...] in Keras Dense convention, one
     pair per layer (keras_model.py:87-101): tanh on all layers but the last,
     which is linear and has V outputs.  The first kernel has He+Hd rows.
+    dropout: rate behind every tanh (training), with the mask that
+    ``rnnt_amd.dropout`` draws for [B,T,U+1,H] at seed and offset + layer, so a
+    step uses the offsets offset .. offset + len(weights) - 2; offset may be an
+    int64 on the device.  0: none.
     Returns acts[B,T,U+1,V]."""
     if len(weights) < 1:
         raise ValueError("fc_joint: at least one Dense layer")
+    drop16("fc_joint", dropout)  # refuses a rate outside [0, 1)
     He = y_trans.shape[2]
     k1, b1 = weights[0]
     if k1.shape[0] != He + y_pred.shape[2]:
@@ -146,26 +155,35 @@ def fc_joint(y_trans, y_pred, weights):
     if len(weights) == 1:                           # linear single layer: an additive joint
         return pe.unsqueeze(2) + pd.unsqueeze(1)
     h = fc_joint_first_layer(pe, pd)
-    for k, b in weights[1:-1]:
-        h = joint_dense(h, k, b, "tanh")
+    if dropout:
+        h = _dropout(h, dropout, seed, offset)
+        for i, (k, b) in enumerate(weights[1:-1]):
+            at = offset + i + 1 if isinstance(offset, torch.Tensor) else (int(offset) + i + 1) % 2 ** 64
+            h = dense(h, k.float(), b.float(), "tanh", dropout=dropout, seed=seed, offset=at)
+    else:
+        for k, b in weights[1:-1]:
+            h = joint_dense(h, k, b, "tanh")
     k, b = weights[-1]
     return joint_dense(h, k, b, "linear")
 
 
-def fc_joint_loss(y_trans, y_pred, weights, labels, input_length, label_length, blank_label=REFERENCE_BLANK_LABEL):
+def fc_joint_loss(y_trans, y_pred, weights, labels, input_length, label_length, blank_label=REFERENCE_BLANK_LABEL, dropout=0.0, seed=0, offset=0):
     """The loss of the FC-joint model from the two network outputs:
     rnnt_lambda_func_v2([get_fc(concatenate_lambda([y_trans, y_pred])), labels,
     input_length, label_length]) (keras_model.py:169-188) -> costs[B].
     The first SHIFT frames are dropped before the joint instead of after it
-    (every layer acts per position, so the result is the same)."""
+    (every layer acts per position, so the result is the same).  dropout, seed,
+    offset: as fc_joint takes them (the mask's rows are those of the cropped
+    lattice)."""
     B = y_trans.shape[0]
+    drop16("fc_joint_loss", dropout)
     if len(weights) == 1:
         He = y_trans.shape[2]
         k1, b1 = weights[0]
         f = torch.matmul(y_trans, k1[:He])
         g = torch.matmul(y_pred, k1[He:]) + b1
         return rnnt_lambda_func([f, g, labels, input_length, label_length], blank_label=blank_label, fused=True)
-    acts = fc_joint(y_trans[:, SHIFT:], y_pred, weights)
+    acts = fc_joint(y_trans[:, SHIFT:], y_pred, weights, dropout, seed, offset)
     il = (input_length - SHIFT).reshape(B)
     ll = label_length.reshape(B)
     return rnnt_loss(acts, labels, il, ll, blank_label, inplace=True).reshape(B)

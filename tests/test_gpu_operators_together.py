@@ -1,0 +1,100 @@
+"""The operators as they are used together: a training step of the fully-connected joint with dropout against float64, and a
+decoder's steps (dense on the beam's rows, selection, states in their new order) against the float64 checker."""
+import numpy as np
+import pytest
+import torch
+
+import rnnt_amd
+from oracle import operators as ops
+from oracle import rnnt_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def _joint(seed, B, T, U, He, Hd, widths, V):
+    g = torch.Generator().manual_seed(seed)
+    def t(*s, scale=1.0):
+        return torch.randn(s, generator=g) * scale
+    yt, yp = t(B, T, He), t(B, U + 1, Hd)
+    sizes = [He + Hd, *widths, V]
+    weights = [(t(a, b, scale=a ** -0.5), t(b, scale=0.1)) for a, b in zip(sizes, sizes[1:])]
+    lab = torch.randint(0, V - 1, (B, U), generator=g, dtype=torch.int32)
+    return yt, yp, weights, lab
+
+
+@pytest.mark.parametrize("widths", [(24,), (40, 30), (150, 33, 20)])
+def test_training_step_of_the_joint_with_dropout(widths):
+    B, T, U, He, Hd, V, rate, seed, offset = 2, 9, 4, 20, 12, 17, 0.3, 5, 2 ** 40
+    yt, yp, weights, lab = _joint(1, B, T, U, He, Hd, widths, V)
+    il, ll = torch.tensor([[9], [7]], dtype=torch.int32), torch.tensor([[4], [2]], dtype=torch.int32)
+    dev = [t.to(DEV).requires_grad_(True) for t in (yt, yp, *[w for p in weights for w in p])]
+    pairs = list(zip(dev[2::2], dev[3::2]))
+    costs = rnnt_amd.fc_joint_loss(dev[0], dev[1], pairs, lab.to(DEV), il.to(DEV), ll.to(DEV), blank_label=V - 1, dropout=rate, seed=seed, offset=offset)
+    grads = torch.autograd.grad(costs.mean(), dev)
+
+    # float64 on the host: the joint by autograd with the masks as constants, the loss and its gradient by the oracle
+    ref = [t.double().requires_grad_(True) for t in (yt, yp, *[w for p in weights for w in p])]
+    h = torch.cat([ref[0][:, 2:].unsqueeze(2).expand(-1, -1, U + 1, -1), ref[1].unsqueeze(1).expand(-1, T - 2, -1, -1)], dim=-1)
+    for i, (k, b) in enumerate(zip(ref[2::2], ref[3::2])):
+        h = h @ k + b
+        if i < len(weights) - 1:
+            h = torch.tanh(h)
+            m = ops.dropout_scale(B * (T - 2) * (U + 1), h.shape[-1], rate, seed, offset + i)
+            h = h * torch.from_numpy(m).reshape(h.shape)
+    want, d_acts = orc.rnnt_loss_and_grad(h.detach().numpy(), lab.numpy(), (il - 2).reshape(B).numpy(), ll.reshape(B).numpy(), V - 1, np.full(B, 1.0 / B))
+    np.testing.assert_allclose(costs.detach().cpu().numpy(), want, rtol=1e-5)
+    for g, r in zip(grads, torch.autograd.grad(h, ref, torch.from_numpy(np.asarray(d_acts, np.float64)))):
+        # the loss's own bar on d_acts is 1e-4 absolute (2e-5 measured); a gradient of a weight sums up to B T (U+1) of them
+        assert (g.cpu().double() - r).abs().max() < 1e-4 * max(1.0, r.abs().max().item())
+
+
+def test_no_dropout_is_what_it_was():
+    yt, yp, weights, _ = _joint(2, 2, 6, 3, 10, 8, (20, 12), 9)
+    args = yt.to(DEV), yp.to(DEV), [(k.to(DEV), b.to(DEV)) for k, b in weights]
+    assert torch.equal(rnnt_amd.fc_joint(*args), rnnt_amd.fc_joint(*args, dropout=0.0, seed=3, offset=9))
+    with pytest.raises(ValueError):
+        rnnt_amd.fc_joint(*args, dropout=1.0)
+
+
+def test_an_offset_in_device_memory_gives_the_same_step():
+    yt, yp, weights, _ = _joint(3, 1, 5, 2, 6, 6, (16, 16, 8), 7)
+    args = yt.to(DEV), yp.to(DEV), [(k.to(DEV), b.to(DEV)) for k, b in weights]
+    a = rnnt_amd.fc_joint(*args, dropout=0.5, seed=3, offset=70)
+    assert torch.equal(a, rnnt_amd.fc_joint(*args, dropout=0.5, seed=3, offset=torch.tensor([70], device=DEV)))
+    assert not torch.equal(a, rnnt_amd.fc_joint(*args, dropout=0.5, seed=3, offset=71))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [62, 2500])
+def test_decoder_steps(V, dtype):
+    """Three steps of a beam search over a small recurrent prediction network: hidden layer with a skip connection, output layer,
+    selection, reordering.  The checker selects from the very logits the layers gave, in float64."""
+    g = torch.Generator().manual_seed(4)
+    B, K, H = 3, 4, 48
+    def t(*s, scale=1.0):
+        return (torch.randn(s, generator=g) * scale).to(dtype).to(DEV)
+    w1, b1, w2, b2, emb, enc = t(H, H, scale=H ** -0.5), t(H, scale=0.1), t(H, V, scale=2 * H ** -0.5), t(V, scale=0.1), t(V, H), t(B, V)
+    h = t(B, 1, H).expand(B, K, H)
+    scores = torch.full((B, K), float("-inf"), device=DEV)
+    scores[:, 0] = 0
+    finished = torch.zeros(B, K, dtype=torch.bool, device=DEV)
+    history = torch.zeros(B, K, 3, dtype=torch.int64, device=DEV)
+    for step in range(3):
+        h = rnnt_amd.dense(h, w1, b1, "tanh", residual=h)
+        logits = rnnt_amd.dense(h, w2, b2)
+        args = logits, scores, K
+        new, parent, token = rnnt_amd.beam_select(*args, enc=enc, finished=finished, end=0)
+        want = ops.beam_select(logits.float().cpu().numpy(), scores.cpu().numpy(), K, enc=enc.float().cpu().numpy(), finished=finished.cpu().numpy(), end=0)
+        np.testing.assert_array_equal(parent.cpu().numpy(), want[1])
+        np.testing.assert_array_equal(token.cpu().numpy(), want[2])
+        np.testing.assert_allclose(new.cpu().numpy(), want[0], rtol=2.0 ** -23, atol=2.0 ** -22)
+        before = h.cpu(), history.cpu()
+        h, history = rnnt_amd.beam_reorder(parent, [h, history])
+        at = torch.arange(B)[:, None], parent.cpu().long()
+        assert torch.equal(h.cpu(), before[0][at]) and torch.equal(history.cpu(), before[1][at])
+        history[:, :, step] = token
+        finished = token == 0
+        scores = new
+        h = h + emb[token.long()]
+    assert scores.isfinite().all() and (scores[:, :-1] >= scores[:, 1:]).all()
