@@ -16,6 +16,7 @@ from . import _lib
 from ._operator import check, dtype_code, need_gpu, on_device, stream
 
 MAX_BEAMS = 64
+_INT = 0x7FFFFFFF  # sizes the C entry points take as int
 MAX_WIDTH = 64
 
 
@@ -26,8 +27,8 @@ def beam_select(logits, scores, width, enc=None, allowed=None, finished=None, en
     type, the prediction network's part of an additive joint (logits + enc, rounded to float32, as joint_log_softmax does).
     scores [B, K] float32: log-probabilities so far; -inf, NaN or anything beyond +-2^30 marks an empty beam.
     allowed: bool [V] or [B, V]; a forbidden symbol is no candidate and has no part in the softmax, whatever its logit.
-    finished: bool [B, K]; such a beam is carried along, as one candidate with its own score at symbol `end` (in a
-    transducer: a hypothesis that has emitted blank and waits for the next frame).
+    finished: bool [B, K]; such a beam is carried along, as one candidate with its own score at symbol `end`, allowed or not (in
+    a transducer: a hypothesis that has emitted blank and waits for the next frame).  Nothing is differentiable here.
 
     Returns scores [B, width] float32, parent [B, width] int32 (beam) and token [B, width] int32, in descending order of
     scores + log_softmax (compared in float64), ties to the lowest beam, then the lowest symbol.  Where there are fewer
@@ -40,6 +41,8 @@ def beam_select(logits, scores, width, enc=None, allowed=None, finished=None, en
     width = int(width)
     if not 1 <= width <= MAX_WIDTH or K > MAX_BEAMS:
         raise ValueError(f"beam_select: 1 to {MAX_WIDTH} continuations of at most {MAX_BEAMS} beams, got {width} of {K}")
+    if K * V > _INT or B > _INT:
+        raise ValueError(f"beam_select: beams x vocabulary must stay below 2^31, got {tuple(logits.shape)}")
     if scores.shape != (B, K) or scores.dtype != torch.float32:
         raise ValueError("beam_select: scores must be float32 [B, K]")
     if enc is not None and (enc.shape != (B, V) or enc.dtype != logits.dtype):
@@ -130,6 +133,8 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
         for i, (a0, a1, written) in enumerate(spans):
             if written and any(a0 < b1 and b0 < a1 for j, (b0, b1, _) in enumerate(spans) if j != i):
                 raise ValueError("beam_reorder: out overlaps a state, another output or parent")
+    if max(B, K, W) > _INT:
+        raise ValueError("beam_reorder: more than 2^31 - 1 utterances or beams")
     if K == 0:
         for o in out:
             o.zero_()

@@ -437,21 +437,29 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
   const int lists_here = a.K * a.pieces;
   lists += (long long)b * lists_here * P;
+  // everything that the first half needs is asked for at once
+  const int first = wave * 64 + lane;
+  RowKey head = {0u, 0u};
+  if (first < lists_here) head = lists[(long long)first * P];
   for (int k = wave; k < a.K; k += waves) {
     const long long row = (long long)b * a.K + k;
-    float score = a.scores[row];
+    const PieceSum* mine = sums + row * a.pieces;
+    const float given = a.scores[row];
     const bool done = a.finished && a.finished[row];
+    PieceSum q = {0.0, -INFINITY, 0.f};
+    if (lane < a.pieces) q = mine[lane];
+    float score = given;
     RowSum of = {0.0, 0.0};
     if (!live_score(score)) score = NAN;
     else if (!done) {  // uniform
-      float m = -INFINITY;
-      for (int p = lane; p < a.pieces; p += 64) m = fmaxf(m, sums[row * a.pieces + p].m);
+      float m = q.m;
+      for (int p = lane + 64; p < a.pieces; p += 64) m = fmaxf(m, mine[p].m);
       m = wave_max(m);
-      double s = 0.0;
-      for (int p = lane; p < a.pieces; p += 64) {
-        const PieceSum q = sums[row * a.pieces + p];
-        // a piece without an allowed symbol has m = -inf and s = 0; a NaN sum stays one
-        s += q.m == -INFINITY ? q.s : q.s * exp((double)q.m - (double)m);
+      // a piece without an allowed symbol has m = -inf and s = 0; a NaN sum stays one
+      double s = q.m == -INFINITY ? q.s : q.s * exp((double)q.m - (double)m);
+      for (int p = lane + 64; p < a.pieces; p += 64) {
+        const PieceSum o = mine[p];
+        s += o.m == -INFINITY ? o.s : o.s * exp((double)o.m - (double)m);
       }
       s = wave_sum(s);
       of = RowSum{(double)m, log(s)};
@@ -464,17 +472,17 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
     }
   }
   __syncthreads();
-  auto entry = [&](int l, int r) {  // the r-th candidate of list l
+  auto entry = [&](int l, int r, const RowKey& c) {  // the r-th candidate of list l, which is c
     const int k = l / a.pieces;
     const float score = live[k];
     if (score != score) return TotalKey{0ull, 0u};
-    if (!over[k]) return total_key(a, k, false, score, rows[k], lists[(long long)l * P + r]);
+    if (!over[k]) return total_key(a, k, false, score, rows[k], c);
     return r == 0 && l == k * a.pieces ? total_key(a, k, true, score, rows[k], RowKey{0u, 0u}) : TotalKey{0ull, 0u};
   };
   TotalKey heads = {0ull, 0u};
-  for (int l0 = wave * 64; l0 < lists_here; l0 += waves * 64) {
+  for (int l = first; l - lane < lists_here; l += waves * 64) {
     TotalKey t = {0ull, 0u};
-    if (l0 + lane < lists_here) t = entry(l0 + lane, 0);
+    if (l < lists_here) t = entry(l, 0, l == first ? head : lists[(long long)l * P]);
     if (__any(t.hi != 0)) {
       sort64(t, lane);
       join<64>(heads, lane_xor<63>(t), lane);
@@ -492,7 +500,8 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
     const int w = l0 + lane / P;
     if (w < a.width && best[w].hi) {
       const uint32_t flat = ~best[w].lo, k = flat / (uint32_t)a.V;
-      t = entry((int)k * a.pieces + (over[k] ? 0 : (int)(flat - k * (uint32_t)a.V) / kPiece), r);
+      const int l = (int)k * a.pieces + (over[k] ? 0 : (int)(flat - k * (uint32_t)a.V) / kPiece);
+      t = entry(l, r, over[k] ? RowKey{0u, 0u} : lists[(long long)l * P + r]);
     }
     join<P>(acc, t, lane);
   }

@@ -482,7 +482,7 @@ int check_layer(const rnnt_mi355x_layer* l) {
     return RNNT_MI355X_INVALID_VALUE;
   // 32-bit indexes inside an operand's rows and of its tiles
   if (l->rows > 0x7fff0000ll || l->in > (1 << 24) || l->out > (1 << 24) || ((l->rows + 63) / 64) * ((l->in + 63) / 64) > 0x7fffffffll ||
-      ((l->rows + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll)
+      ((l->rows + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll || (long long)((l->in + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll)
     return RNNT_MI355X_UNSUPPORTED_SIZE;
   return RNNT_MI355X_OK;
 }

@@ -358,7 +358,7 @@ struct GemmArgs {
 template <bool A_KS, bool B_KS>
 __device__ __forceinline__ float product_again(const float* a, const float* b, long long a_ld, long long b_ld, long long m, int n, int k0, int k1) {
   float s = 0.f;
-  for (int k = k0; k < k1; ++k)
+  for (int k = k0; k < k1 && s == s; ++k)  // once no number, always none
     s = fmaf(A_KS ? a[(long long)k * a_ld + m] : a[m * a_ld + k], B_KS ? b[(long long)k * b_ld + n] : b[(long long)n * b_ld + k], s);
   return s;
 }
@@ -699,7 +699,7 @@ __device__ __forceinline__ void gemm_ring(const GemmArgs& g, int id, char* lds0,
     step(buf3, buf0, buf2);
     if (--left == 0) break;
   }
-  __syncthreads();  // also waits for the tiles past the end, which are still on their way
+  landed<0>();  // also the tiles past the end, which were still on their way
   if constexpr (GROUPS > 1) {
     static_assert(kSums<IM, IN, kThreads> <= kStage * GROUPS && kThreads / 64 * kWayOut<IN> <= kStage * GROUPS, "");
     char* const place[GROUPS] = {lds0, lds1, lds2, lds3};

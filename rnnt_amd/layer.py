@@ -14,6 +14,7 @@ from . import _lib
 from ._operator import DTYPE_CODE, check, drop16, dtype_code, need_gpu, on_device, seed_offset, stream
 
 ACTIVATIONS = {"linear": 0, "tanh": 1, "relu": 2, "gelu": 3, "silu": 4}
+MAX_WIDTH = 1 << 24  # inputs and outputs of rnnt_mi355x_layer_*
 _AUX_TYPE = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 
 
@@ -126,6 +127,8 @@ def dense(x, kernel, bias=None, activation="linear", residual=None, dropout=0.0,
         raise ValueError(f"dense: activation must be one of {', '.join(ACTIVATIONS)}")
     if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0] or 0 in kernel.shape:
         raise ValueError(f"dense: x{tuple(x.shape)} does not fit kernel{tuple(kernel.shape)}")
+    if max(kernel.shape) > MAX_WIDTH:
+        raise ValueError(f"dense: a layer is at most {MAX_WIDTH} wide, got kernel{tuple(kernel.shape)}")
     if bias is not None and bias.shape != kernel.shape[1:]:
         raise ValueError(f"dense: bias{tuple(bias.shape)} does not fit kernel{tuple(kernel.shape)}")
     if residual is not None and residual.shape != x.shape[:-1] + kernel.shape[1:]:

@@ -15,6 +15,8 @@ from ._operator import DTYPE_CODE, check, drop16, dtype_code, need_gpu, on_devic
 
 def _apply(x, drop, seed, offset, offset_t):
     cols = stride = x.shape[-1]
+    if cols > 0x7FFFFFFF:  # the C entry point takes it as an int
+        raise ValueError("dropout: the last dimension holds 2^31 elements or more")
     if x.is_contiguous():
         y = torch.empty_like(x)
     else:

@@ -172,8 +172,9 @@ def test_infinities_overflow_and_nan(shape):
     w[0, :3] = 1.0
     x[5], x[6], w[:, 4] = 1e-38, 1e38, 1e-30
     got = rnnt_amd.dense(x.to(DEV), w.to(DEV)).cpu().double().numpy()
+    x, w = x.numpy(), w.numpy()
     with np.errstate(all="ignore"):
-        want = x.double().numpy() @ w.double().numpy()
+        want = x.astype(np.float64) @ w.astype(np.float64)
         over = np.abs(want) > 3.4028235e38
     ok = np.isfinite(want) & ~over
     assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
@@ -185,6 +186,12 @@ def test_infinities_overflow_and_nan(shape):
     one = lambda t, axis: np.abs(np.where(np.isfinite(t), t, 0).astype(np.float64)).sum(axis, keepdims=True)  # noqa: E731
     least = 2.0 ** -125 * (one(w, 0) + one(x, 1))
     assert (np.abs(got - want)[fine] <= (acc(K, s) + 2.0 ** -24 * np.abs(want) + least)[fine]).all()
+
+
+def test_everything_nan_ends_soon():
+    """A diverged model: every float32 result is computed again, which ends at the first value that is no number."""
+    x = torch.full((3000, 20000), float("nan"), device=DEV)
+    assert rnnt_amd.dense(x, torch.ones(20000, 300, device=DEV)).isnan().all()
 
 
 @pytest.mark.parametrize("act", ["tanh", "relu", "gelu", "silu"])
