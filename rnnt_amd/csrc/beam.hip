@@ -14,7 +14,9 @@
 //   - sorted lists are joined by the first step of a bitonic merge: of two sorted lists a, b the values
 //     max(a[i], b[P-1-i]) are the P largest, and log2 P exchanges sort them.
 // Rows of up to 2048 symbols take one launch, a block per utterance; longer ones a launch over pieces of 2048 and one that
-// joins the pieces' lists.
+// joins the pieces' lists.  Measured, 32 utterances x 16 beams x 32003 symbols in bfloat16 with a mask: pieces 17.5 us (34 MB;
+// half of it are the 27 instructions a symbol), join 9.8 us; 4 x 32 x 65536 in float16 without one: 11 and 15 us; 64 x 8 x 1024
+// in float32: 8.6 us.  The joins, and the short rows, are chains of latencies: sorting networks over a wavefront, LDS, memory.
 #include "op_util.h"
 
 namespace {
@@ -568,8 +570,8 @@ struct ReorderArgs {
 };
 constexpr int kRowPiece = 4096;  // bytes of a row that one wavefront copies: four 16-byte loads a lane
 
-// A wavefront per piece of a row: bound by memory, or by the launch for the states of a single utterance; all tensors of a
-// step go in one launch.
+// A wavefront per piece of a row: bound by memory, or by the launch for the states of a single utterance (4 us); all tensors of
+// a step go in one launch.
 __global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a, unsigned items) {
   const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;

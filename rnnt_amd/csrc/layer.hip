@@ -89,7 +89,8 @@ __global__ __launch_bounds__(256) void k_layer_pack(PackArgs a, PackArgs b) {
 }
 
 // dz, its column sums, and the copies of the operands that lie badly: what the gradient's products begin with.  Bound by
-// memory: dy and the saved tensor read once, dz written once.
+// memory, dy and the saved tensor read once and dz written once (49200 x 250 float32, tanh and dropout: 28 us = 5.3 TB/s), or by
+// the slope and the generator where elements are small (32768 x 4096 bfloat16, gelu and dropout: 185 us = 4.3 TB/s).
 template <class T>
 __global__ __launch_bounds__(kDzGroups * kDzLanes) void k_layer_dz(DzArgs a, PackArgs p, PackArgs q) {
   static_assert(kDzGroups * kDzLanes == 256, "pack_block's size");
@@ -218,6 +219,7 @@ constexpr int kRowsVec = T::code == RNNT_MI355X_FP32 ? 1 : 2;  // columns a lane
 // x W for at most 8 rows: bound by the read of W, or by a launch and a few memory latencies for a small one, where the
 // matrix cores' tiles of 32 rows would be mostly empty.  A block has 64 or 128 columns; its 16 wavefronts share k, each reads
 // its rows of W straight into registers, 16 at a time, and takes x from LDS.  The sums of the wavefronts meet in LDS.
+// 8 x 250 x 62 float32: 6.0 us of the GPU, the matrix cores' block of 32 rows 13.6.
 template <class T, int MR>
 __global__ __launch_bounds__(64 * kRowsSlices) void k_layer_rows(GemmArgs g) {
   using E = typename T::elem;

@@ -185,7 +185,8 @@ def test_infinities_overflow_and_nan(shape):
     # before, so what is dropped of it is below 2^-126 (1 + 2^-8 + 2^-16), less than 2^-125, times the other operand.
     one = lambda t, axis: np.abs(np.where(np.isfinite(t), t, 0).astype(np.float64)).sum(axis, keepdims=True)  # noqa: E731
     least = 2.0 ** -125 * (one(w, 0) + one(x, 1))
-    assert (np.abs(got - want)[fine] <= (acc(K, s) + 2.0 ** -24 * np.abs(want) + least)[fine]).all()
+    got, want = got[fine], want[fine]
+    assert (np.abs(got - want) <= acc(K, s)[fine] + 2.0 ** -24 * np.abs(want) + least[fine]).all()
 
 
 def test_everything_nan_ends_soon():
@@ -209,12 +210,14 @@ def test_far_pre_activations(act, dtype):
     a[-3], a[-2] = {"tanh": (1, -1)}.get(act, (np.inf, 0))
     s[-3], s[-2] = (0, 0) if act == "tanh" else (1, 0)
     got_a, got_s = f64(y)[:, 0], f64(dx)[:, 0]
+    a[-1] = s[-1] = 0  # the value that is no number has its own line
     assert np.isnan(got_a[-1]) and (np.isnan(got_s[-1]) or act == "relu")
     assert got_a[-3] == a[-3] and got_a[-2] == a[-2]
     # silu(-400) = -400 e^-400 is no float32: below the smallest normal number, 2^-126, a result may be zero
-    lim = U[dtype] * np.abs(a) + (2.0 ** -21 if act != "gelu" or dtype == torch.float32 else 2.0 ** -19) * np.maximum(1, np.abs(f)) * (np.abs(f) < 100) + np.maximum(LEAST[dtype], 2.0 ** -126)
-    assert (np.abs(got_a - a)[:-3] <= lim[:-3]).all()
-    assert (np.abs(got_s - s)[:-1] <= U[dtype] + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 0)).all()
+    f = np.where(np.isfinite(f), f, 0)
+    lim = U[dtype] * np.where(np.isfinite(a), np.abs(a), 0) + (2.0 ** -21 if act != "gelu" or dtype == torch.float32 else 2.0 ** -19) * np.maximum(1, np.abs(f)) * (np.abs(f) < 100) + np.maximum(LEAST[dtype], 2.0 ** -126)
+    assert (np.abs(got_a[:-3] - a[:-3]) <= lim[:-3]).all()
+    assert (np.abs(got_s[:-1] - s[:-1]) <= U[dtype] + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 0)).all()
 
 
 def test_gradients_against_differences():
