@@ -139,6 +139,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The operators' torch binding (csrc/torch_binding.cpp), calling the library that lib() has loaded."""
+    global _native
+    if _native is None:
+        handle = lib()
+        if _build.needs_native_build():
+            try:
+                _build.build_native()
+            except (RuntimeError, OSError, subprocess.CalledProcessError) as e:
+                raise RNNTLibraryError(f"{_build.NATIVE} is missing or older than its source and building it failed: {e}; build it with "
+                                       "`python -m rnnt_amd.build`") from e
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RNNTLibraryError(f"cannot load {_build.NATIVE}: {e}") from e
+        module.bind({name: ctypes.cast(getattr(handle, name), _vp).value for name in _SIGNATURES})
+        _native = module
+    return _native
+
+
 def status_string(rc: int) -> str:
     return lib().rnnt_mi355x_status_string(int(rc)).decode()
 

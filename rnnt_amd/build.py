@@ -1,4 +1,4 @@
-"""Compiles rnnt_amd/csrc/*.hip into librnnt_mi355x.so for gfx950.
+"""Compiles rnnt_amd/csrc/*.hip into librnnt_mi355x.so for gfx950, and torch_binding.cpp into _native.so.
 
 hipcc cross-compiles without a GPU, so this runs in a CPU-only container; the
 built library stays in-tree (git-ignored) and travels with the source tree.
@@ -21,6 +21,9 @@ PIECES = [os.path.join(CSRC, n) for n in ("workspace.h", "device_util.h", "lse_r
                                           "small_vocab.h", "joint.h", "aux_kernels.h")]
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "rnnt_mi355x.h")
 LIB = os.path.join(CSRC, "librnnt_mi355x.so")
+# the operators' path from torch to the library (plain C++, against the torch that is installed)
+BINDING = os.path.join(CSRC, "torch_binding.cpp")
+NATIVE = os.path.join(_HERE, "_native.so")
 # hipcc's packed float32 instructions have given wrong results on this hardware now and then: no source is built with them
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Xclang", "-target-feature", "-Xclang",
          "-packed-fp32-ops"]
@@ -57,6 +60,55 @@ def newer_sources():
         return [*SOURCES, *OPERATOR_SOURCES]
     t = os.path.getmtime(LIB)
     return [p for p in (*SOURCES, *PIECES, *OPERATOR_SOURCES, *OPERATOR_PIECES, HEADER) if os.path.getmtime(p) > t]
+
+
+def needs_native_build() -> bool:
+    if not os.path.exists(NATIVE):
+        return True
+    t = os.path.getmtime(NATIVE)
+    return any(os.path.getmtime(p) > t for p in (BINDING, HEADER))
+
+
+def native_command(out: str):
+    """The g++ line that compiles the torch binding."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    rocm = os.path.dirname(os.path.dirname(hipcc_path()))
+    if not os.path.isdir(os.path.join(rocm, "include", "hip")):
+        rocm = "/opt/rocm"
+    cxx = shutil.which("g++")
+    if not cxx:
+        raise RuntimeError("g++ not found: cannot build the torch binding")
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"),
+               sysconfig.get_path("include")]
+    # the HIP headers and torch's want to be told their platform
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include], BINDING, "-o", out,
+            f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+
+
+def build_native(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the torch binding; as build(), one process at a time and moved into place when whole."""
+    import fcntl
+    import tempfile
+    if not force and not needs_native_build():
+        return NATIVE
+    with open(NATIVE + ".lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        try:
+            if force or needs_native_build():
+                with tempfile.TemporaryDirectory(prefix=".build-", dir=_HERE) as tmp:
+                    staged = os.path.join(tmp, os.path.basename(NATIVE))
+                    cmd = native_command(staged)
+                    if verbose:
+                        print(" ".join(cmd))
+                    subprocess.check_call(cmd)
+                    os.replace(staged, NATIVE)
+        finally:
+            fcntl.flock(lock, fcntl.LOCK_UN)
+    return NATIVE
 
 
 def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB) -> str:
@@ -102,3 +154,4 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB
 
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
+    print(build_native(force=True, verbose=True))
