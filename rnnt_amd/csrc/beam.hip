@@ -59,7 +59,7 @@ struct RowKey {  // value of a row, then the lower symbol
 struct TotalKey {  // total in float64, then the lower place in beams x vocabulary
   uint64_t hi;
   uint32_t lo;
-  __device__ __forceinline__ bool operator>(const TotalKey& o) const { return hi > o.hi || (hi == o.hi && lo > o.lo); }
+  __device__ __forceinline__ bool operator>(const TotalKey& o) const { return (hi > o.hi) | ((hi == o.hi) & (lo > o.lo)); }  // no branch
 };
 template <int M>
 __device__ __forceinline__ RowKey lane_xor(const RowKey& k) {
