@@ -316,3 +316,17 @@ def test_refusals():
                      ((x, w, torch.zeros(6, device=DEV).half()), {})):
         with pytest.raises(TypeError):
             rnnt_amd.dense(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["tanh", "gelu", "silu"])
+@pytest.mark.parametrize("rows", [8, 400])
+def test_activations_of_small_numbers_are_relative(dtype, act, rows):
+    """With one input and a kernel of ones z is x itself, and the result's error is relative to it: 2^-20 for tanh's formula; Phi
+    and the logistic function are 1/2 + O(z), off by 1.5e-6 < 2^-18 of that at most; half a step for the type."""
+    z = torch.logspace(-36 if dtype != torch.float16 else -7, 0, rows, dtype=torch.float64).to(dtype)
+    z[1::2] *= -1
+    y = rnnt_amd.dense(z.to(DEV)[:, None], torch.ones(1, 9, dtype=dtype, device=DEV), None, act)
+    want = orc.activation(f64(z), act)[0][:, None]
+    tol = (2.0 ** -18 + U[dtype] * 1.01) * np.abs(want) + 2 * LEAST[dtype] + 2.0 ** -125
+    assert (np.abs(f64(y) - want) <= tol).all()
