@@ -5,8 +5,10 @@
 // 6151 x 515 x 1030 in float16 139 and 87.  The entry points are those of the library that rnnt_amd._lib has loaded; their addresses come from there.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/rnnt_mi355x.h"
@@ -74,6 +76,26 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+// Where a backward pass is captured, autograd makes the stream of every node behind this one wait for the stream captured.  A
+// leaf that an eager graph still uses has its node on that graph's stream, and such a wait from outside the capture ends the
+// process; it is refused before it happens.
+void refuse_waits_outside_capture(const char* op) {
+  const auto here = c10::hip::getCurrentHIPStream();
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  for (uint32_t i = 0; node && i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!next || !node->task_should_compute_output(i)) continue;
+    const auto there = next->stream();
+    if (!there || (there->id() == here.id() && there->device_index() == here.device_index())) continue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *there).stream();
+    const bool captured = other && hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+    TORCH_CHECK(captured, op, ": this backward pass is being captured, and goes on to a tensor that an eager graph on another stream still holds; "
+                          "drop that graph and its results first, or give the captured pass leaves of its own");
+  }
+}
+
 constexpr int64_t kInt = 0x7fffffff;  // what an int of the C ABI holds
 
 // ---- dropout ------------------------------------------------------------------------------------------------------------
@@ -109,6 +131,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     return run_dropout(x, Drop{drop16, seed, offset}, offset_t);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    refuse_waits_outside_capture("dropout");
     const auto saved = ctx->get_saved_variables();
     const OptTensor offset_t = saved.empty() ? OptTensor() : OptTensor(saved[0]);
     const Drop d{ctx->saved_data["drop16"].toInt(), ctx->saved_data["seed"].toInt(), ctx->saved_data["offset"].toInt()};
@@ -215,6 +238,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dys) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "dense: the gradient is not differentiable (create_graph)");
+    refuse_waits_outside_capture("dense");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x_given = saved[0], &kernel_given = saved[1], &y = saved[2], &aux = saved[3], &offset_t = saved[4];
     // edges are counted over the tensors that were there

@@ -1,5 +1,7 @@
 """The operators as they are used together: a training step of the fully-connected joint with dropout against float64, and a
 decoder's steps (dense on the beam's rows, selection, states in their new order) against the float64 checker."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -98,3 +100,32 @@ def test_decoder_steps(V, dtype):
         scores = new
         h = h + emb[token.long()]
     assert scores.isfinite().all() and (scores[:, :-1] >= scores[:, 1:]).all()
+
+
+def test_captured_backward_pass_of_leaves_that_an_eager_graph_holds_is_refused():
+    """It would make a stream outside the capture wait for it; with the eager graph gone the same leaves are captured."""
+    x = torch.randn(40, 24, device=DEV)
+    w, b = (torch.randn(24, 16, device=DEV) * 0.2).requires_grad_(True), torch.zeros(16, device=DEV, requires_grad=True)
+
+    def step(k):
+        y = rnnt_amd.dropout(rnnt_amd.dense(x, k, b, "tanh"), 0.25, seed=3)
+        return torch.autograd.grad((y * y).sum(), (k, b))
+    eager = rnnt_amd.dense(x, w, b, "tanh")  # holds the leaves' nodes on this stream
+    with pytest.raises(RuntimeError, match="eager graph on another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step(w)
+    held = rnnt_amd.dropout(w, 0.5)
+    with pytest.raises(RuntimeError, match="eager graph on another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            (rnnt_amd.dropout(w, 0.5) * 2.0).backward(torch.ones_like(w))
+    del eager, held
+    gc.collect()  # and what the errors held
+    want = step(w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(w)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, step(w)))
+    assert all(torch.equal(p, q) for p, q in zip(out, want))
