@@ -278,7 +278,7 @@ int rnnt_mi355x_dropout(const void* x, long long x_stride, void* y, long long ro
  * Workspace: the sizes rnnt_mi355x_layer_workspace_bytes gives for the very pointers
  * and strides (their alignment decides the kernels), on a 256-byte boundary; forward 0:
  * may be NULL.  y may be
- * residual itself when its stride is `out`.  rows < 2^31 - 2^16, in, out <= 2^24. */
+ * residual itself when its stride is `out`.  rows <= 2^30 - 64, in, out <= 2^24. */
 #define RNNT_MI355X_ACT_LINEAR 0
 #define RNNT_MI355X_ACT_TANH 1
 #define RNNT_MI355X_ACT_RELU 2
@@ -310,7 +310,8 @@ int rnnt_mi355x_layer_backward(const rnnt_mi355x_layer* layer, const void* dy, l
  * out_scores / out_parent / out_token [B, width]; places without a candidate hold
  * -inf, -1, -1.  A beam whose score is NaN or beyond +-2^30 is empty; so is one whose
  * allowed logits hold a NaN or +inf, or nothing above -inf.  K, width <= 64,
- * K*V < 2^31.  `workspace`: rnnt_mi355x_beam_select_workspace_bytes
+ * K*V <= 2^31 - 2^16, B < 2^22, B*K*(V/2048 rounded up) < 2^26 where V > 2048.
+ * `workspace`: rnnt_mi355x_beam_select_workspace_bytes
  * on a 16-byte boundary (0: may be NULL). */
 int rnnt_mi355x_beam_select_workspace_bytes(int B, int K, int V, int width, size_t* out_bytes);
 int rnnt_mi355x_beam_select(const void* logits, long long logits_batch_stride, long long logits_beam_stride, int dtype,

@@ -549,8 +549,8 @@ int launch_select_width(const BeamArgs& a, void* workspace, hipStream_t st) {
 
 int check_select(int B, int K, int V, int width) {
   if (B < 1 || K < 1 || V < 1 || width < 1) return RNNT_MI355X_INVALID_VALUE;
-  if (K > kMaxBeams || width > kMaxWidth || (long long)K * V > 0x7fffffffll ||
-      (long long)B * K * ((V + kPiece - 1) / kPiece) > 0x7fffffffll)
+  // a piece's last symbols are counted past V in an int; a launch has fewer than 2^32 threads
+  if (K > kMaxBeams || width > kMaxWidth || (long long)K * V > 0x7fff0000ll || B >= 1 << 22 || (long long)B * K * pieces_of(V) >= 1 << 26)
     return RNNT_MI355X_UNSUPPORTED_SIZE;
   return RNNT_MI355X_OK;
 }
@@ -568,12 +568,13 @@ struct ReorderArgs {
   const int32_t* parent;
   int n, B, K, width;
 };
+constexpr long long kLaunchItems = 1 << 25;
 constexpr int kRowPiece = 4096;  // bytes of a row that one wavefront copies: four 16-byte loads a lane
 
 // A wavefront per piece of a row: bound by memory, or by the launch for the states of a single utterance (4 us); all tensors of
 // a step go in one launch.
-__global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a, unsigned items) {
-  const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a, unsigned first, unsigned items) {
+  const unsigned id = first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (id >= items) return;
   int n = 0;
@@ -676,6 +677,11 @@ extern "C" int rnnt_mi355x_beam_reorder(const rnnt_mi355x_reorder_tensor* tensor
     items += rows * pieces;
     if (items > 0x7fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
   }
-  k_beam_reorder<<<(unsigned)((items + 3) / 4), 256, 0, static_cast<hipStream_t>(hip_stream)>>>(a, (unsigned)items);
-  return hipGetLastError() == hipSuccess ? RNNT_MI355X_OK : RNNT_MI355X_LAUNCH_FAILURE;
+  // a launch has fewer than 2^32 threads
+  for (long long first = 0; first < items; first += kLaunchItems) {
+    const long long n = items - first < kLaunchItems ? items - first : kLaunchItems;
+    k_beam_reorder<<<(unsigned)((n + 3) / 4), 256, 0, static_cast<hipStream_t>(hip_stream)>>>(a, (unsigned)first, (unsigned)(first + n));
+    if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
+  }
+  return RNNT_MI355X_OK;
 }

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kThreads) void k_dropout(const typename T::elem* x,
 
 template <class T>
 int launch(const void* x, void* y, long long rows, int cols, long long x_stride, const DropArgs& a, hipStream_t st) {
-  const uint32_t groups = (uint32_t)((cols + 7) / 8);
+  const uint32_t groups = (uint32_t)(((long long)cols + 7) / 8);
   const uint64_t total = (uint64_t)rows * groups, per = kThreads * kGroups;
   if ((total + per - 1) / per > 0x7fffffffull) return RNNT_MI355X_UNSUPPORTED_SIZE;
   // the block's first group is below `groups`, so v < groups + 1024

@@ -482,8 +482,8 @@ int check_layer(const rnnt_mi355x_layer* l) {
   if (!l || l->rows < 1 || l->in < 1 || l->out < 1 || l->dtype < 0 || l->dtype > RNNT_MI355X_FP16 || l->act < kLinear || l->act > kSilu ||
       l->drop16 < 0 || l->drop16 > 65535 || l->x_stride < l->in || l->kernel_stride < l->out)
     return RNNT_MI355X_INVALID_VALUE;
-  // 32-bit indexes inside an operand's rows and of its tiles
-  if (l->rows > 0x7fff0000ll || l->in > (1 << 24) || l->out > (1 << 24) || ((l->rows + 63) / 64) * ((l->in + 63) / 64) > 0x7fffffffll ||
+  // 32-bit indexes inside an operand's rows and of its tiles; a launch has fewer than 2^32 threads: 2^24 tiles of 64 rows
+  if (l->rows > (1ll << 30) - 64 || l->in > (1 << 24) || l->out > (1 << 24) || ((l->rows + 63) / 64) * ((l->in + 63) / 64) > 0x7fffffffll ||
       ((l->rows + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll || (long long)((l->in + 63) / 64) * ((l->out + 63) / 64) > 0x7fffffffll)
     return RNNT_MI355X_UNSUPPORTED_SIZE;
   return RNNT_MI355X_OK;
@@ -495,9 +495,6 @@ int saved_by(const rnnt_mi355x_layer* l) {
   const bool from_y = !l->residual && (l->act == kRelu || (l->act == kTanh && l->dtype == RNNT_MI355X_FP32));
   return from_y && l->y ? kOutput : -1;
 }
-
-// row blocks of the dz pass: at most 1024 partial sums a column
-int dz_rows(long long M) { return M <= 65536 ? 64 : (int)((M + 1023) / 1024 + 7) / 8 * 8; }
 
 // Rows in the workspace: whole 16-byte pieces, and no multiple of 4 KiB apart, which puts the same piece of all rows of a
 // tile into the same few memory channels: 32768 x 4096 x 1024 in bfloat16 ran 300 us with such rows of x and 257 us with
@@ -516,10 +513,10 @@ struct Operand {
   size_t at, bytes;
 };
 // Copying costs a read and a write of the operand; the product reads it at twice the speed or better.  6151 x 515 x 1030 in
-// float16, forward: 46 us from the rows as they are, 21 us copies included.  Operands that few rows use stay where they are.
+// float16, forward: 46 us from the rows as they are, 21 us copies included.  Operands that few rows use stay where they are, and those of 2^33 elements.
 Operand operand(const void* p, long long ld, long long rows, int cols, int dtype, bool often) {
   Operand o{p, ld, rows, cols, false, 0, 0};
-  if (dtype != RNNT_MI355X_FP32 && often && !can_go_direct(p, ld, cols, dtype) && cols < (1 << 20)) {
+  if (dtype != RNNT_MI355X_FP32 && often && !can_go_direct(p, ld, cols, dtype) && cols < (1 << 20) && rows * ((cols + 7) / 8) < 1ll << 30) {
     o.pack = true;
     o.ld = workspace_stride(cols, dtype);
     o.bytes = align_up((size_t)rows * o.ld * 2);
@@ -528,14 +525,12 @@ Operand operand(const void* p, long long ld, long long rows, int cols, int dtype
 }
 bool direct(const Operand& o, int dtype) { return o.pack || can_go_direct(o.p, o.ld, o.cols, dtype); }
 // What copies an operand; afterwards it is its copy.
-int pack_of(Operand& o, long long src_ld, char* ws, PackArgs* p) {
-  *p = PackArgs{static_cast<const uint16_t*>(o.p), reinterpret_cast<uint16_t*>(ws + o.at), src_ld, o.ld, o.rows, o.cols, 0u};
-  if (!o.pack) return RNNT_MI355X_OK;
-  const long long n = (o.rows * ((o.cols + 7) / 8) + 255) / 256;
-  if (n > 0x3fffffffll) return RNNT_MI355X_UNSUPPORTED_SIZE;
-  p->blocks = (unsigned)n;
+PackArgs pack_of(Operand& o, long long src_ld, char* ws) {
+  PackArgs p{static_cast<const uint16_t*>(o.p), reinterpret_cast<uint16_t*>(ws + o.at), src_ld, o.ld, o.rows, o.cols, 0u};
+  if (!o.pack) return p;
+  p.blocks = (unsigned)((o.rows * ((o.cols + 7) / 8) + 255) / 256);
   o.p = ws + o.at;
-  return RNNT_MI355X_OK;
+  return p;
 }
 
 constexpr int kOften = 512;  // rows that share the kernel
@@ -607,16 +602,13 @@ int forward(const rnnt_mi355x_layer* l, ForwardPlan f, void* workspace, hipStrea
   e.act = l->act;
   e.drop = drop_args(l->drop16, l->seed, l->offset, l->offset_dev);
   char* ws = static_cast<char*>(workspace);
-  PackArgs px, pk;
-  int rc = pack_of(f.x, l->x_stride, ws, &px);
-  if (rc == RNNT_MI355X_OK) rc = pack_of(f.kernel, l->kernel_stride, ws, &pk);
-  if (rc != RNNT_MI355X_OK) return rc;
+  const PackArgs px = pack_of(f.x, l->x_stride, ws), pk = pack_of(f.kernel, l->kernel_stride, ws);
   if (px.blocks + pk.blocks) {
     k_layer_pack<<<px.blocks + pk.blocks, 256, 0, st>>>(px, pk);
     if (hipGetLastError() != hipSuccess) return RNNT_MI355X_LAUNCH_FAILURE;
   }
   const GemmArgs g = product_args(f.y, f.x.p, f.x.ld, f.kernel.p, f.kernel.ld, (int)l->rows, l->out, l->in, e, ws + f.partial_at);
-  rc = run_product<T>(kForward, f.y, g, st);
+  const int rc = run_product<T>(kForward, f.y, g, st);
   return rc == RNNT_MI355X_OK ? run_join<T>(join_args(f.y, g), no_join(), DbArgs{}, st) : rc;
 }
 
@@ -630,10 +622,7 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
   float* sums = reinterpret_cast<float*>(ws + b.sums_at);
   if (!dx) b.kernel.pack = false;
   if (!dkernel) b.x.pack = false;
-  PackArgs px, pk;
-  int rc = pack_of(b.x, l->x_stride, ws, &px);
-  if (rc == RNNT_MI355X_OK) rc = pack_of(b.kernel, l->kernel_stride, ws, &pk);
-  if (rc != RNNT_MI355X_OK) return rc;
+  const PackArgs px = pack_of(b.x, l->x_stride, ws), pk = pack_of(b.kernel, l->kernel_stride, ws);
   DzArgs a;
   a.dy = dy;
   a.saved = from == kPreActivation ? l->aux : l->y;
@@ -655,6 +644,7 @@ int backward(const rnnt_mi355x_layer* l, const void* dy, long long dy_stride, vo
   }
   const GemmArgs gx = product_args(b.dx, b.dz.p, b.dz.ld, b.kernel.p, b.kernel.ld, M, l->in, l->out, plain_output(dx, l->in), ws + b.partial_at);
   const GemmArgs gk = product_args(b.dk, b.x.p, b.x.ld, b.dz.p, b.dz.ld, l->in, l->out, M, plain_output(dkernel, l->out), ws + b.partial_at + align_up(b.dx.partial_bytes));
+  int rc = RNNT_MI355X_OK;
   if (dx && dkernel && b.dx.block == kBlock128x128 && b.dk.block == kBlock128x128 && b.dx.direct == b.dk.direct) {
     rc = grads_of<T>(b.dx.direct, gx, gk, st);
   } else {

@@ -318,7 +318,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits_given, const
   if (width < 1 || width > kMaxWidth || K > kMaxBeams)
     bad_value("beam_select: 1 to " + std::to_string(kMaxWidth) + " continuations of at most " + std::to_string(kMaxBeams) + " beams, got " +
               std::to_string(width) + " of " + std::to_string(K));
-  if (V > kInt / K || B > kInt) bad_value("beam_select: beams x vocabulary must stay below 2^31, got " + shape(logits));
+  if (V > 0x7fff0000 / K || B > kInt) bad_value("beam_select: beams x vocabulary must not pass 2^31 - 2^16, got " + shape(logits));
   if (scores.dim() != 2 || scores.size(0) != B || scores.size(1) != K || scores.scalar_type() != at::kFloat)
     bad_value("beam_select: scores must be float32 [B, K]");
   if (enc.defined()) {
@@ -416,6 +416,7 @@ std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<T
     Tensor s = states[i];
     const Tensor& o = out[i];
     if (o.numel() == 0) continue;
+    if (s.is_conj() || s.is_neg()) keep.push_back(s = s.resolve_conj().resolve_neg());  // what memory holds is not the value
     if (!s.is_contiguous()) {
       // [outer, B, K, row]: the row has to be dense, the three leading dimensions need one stride each
       bool dense_row = d <= 1;

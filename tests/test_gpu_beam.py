@@ -245,3 +245,13 @@ def test_step_on_another_stream_and_in_a_graph():
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_reorder_of_conjugate_and_negated_views():
+    """Views whose memory does not hold the values they stand for."""
+    s = torch.randn(2, 3, 5, dtype=torch.complex64, device=DEV)
+    parent = torch.tensor([[2, 0], [1, 1]], dtype=torch.int32, device=DEV)
+    index = parent.long()[..., None].expand(2, 2, 5)
+    for v in (s.conj(), s.conj().imag):
+        (got,) = rnnt_amd.beam_reorder(parent, [v])
+        assert torch.equal(got, v.resolve_conj().resolve_neg().gather(1, index))

@@ -65,3 +65,24 @@ def test_reorder_beyond_2_31_bytes():
     (out,) = rnnt_amd.beam_reorder(parent, [states])
     want = torch.arange(40, device=DEV).unsqueeze(1) * 4 + parent
     assert torch.equal(out[:, :, 0].long(), want.long()) and torch.equal(out[:, :, -1].long(), want.long())
+
+
+def test_reorder_of_more_rows_than_a_launch_has_wavefronts():
+    """2^26 rows and some, a wavefront each: a launch holds fewer than 2^32 threads."""
+    B, K, W = (1 << 20) + 3, 5, 64
+    states = torch.randint(0, 256, (B, K), device=DEV, dtype=torch.uint8)
+    parent = torch.randint(-1, K, (B, W), device=DEV, dtype=torch.int32)
+    (out,) = rnnt_amd.beam_reorder(parent, [states])
+    for part in (slice(0, 1000), slice(B // 2 - 500, B // 2 + 500), slice(B - 1000, B)):
+        p = parent[part].long()
+        assert torch.equal(out[part], torch.where(p < 0, 0, states[part].gather(1, p.clamp(min=0))))
+
+
+def test_dropout_of_the_longest_row():
+    n = (1 << 31) - 1
+    x = torch.ones(n, device=DEV, dtype=torch.float16)
+    y = rnnt_amd.dropout(x, 0.25, seed=3, offset=4)
+    groups = np.arange((n + 7) // 8 - 4, (n + 7) // 8, dtype=np.uint64)
+    c = [groups, np.zeros_like(groups), np.full_like(groups, 4), np.zeros_like(groups)]
+    u = np.stack([h for q in orc.philox4x32(c, (3, 0)) for h in (q & np.uint64(0xFFFF), q >> np.uint64(16))], axis=1).reshape(-1)[:31]
+    assert ((y[-31:] > 0).cpu().numpy() == (u >= 16384)).all()

@@ -139,3 +139,22 @@ def test_checker_of_the_mask_keeps_the_right_share():
     kept = (s > 0).sum()
     assert abs(kept - 0.7 * n) < 5 * np.sqrt(n * 0.21)
     assert np.allclose(s[s > 0], 1 / 0.7, rtol=1e-4)
+
+
+def test_beam_select_refuses_a_vocabulary_whose_last_piece_passes_the_int():
+    q, n = _lib.lib().rnnt_mi355x_beam_select_workspace_bytes, ctypes.c_size_t(0)
+    for V in ((1 << 31) - 1, (1 << 31) - 8, (1 << 31) - 2048, (1 << 31) - (1 << 16) + 1):
+        assert q(1, 1, V, 4, ctypes.byref(n)) == _lib.UNSUPPORTED_SIZE
+    assert q(1, 1, (1 << 31) - (1 << 16), 4, ctypes.byref(n)) == 0
+
+
+def test_calls_beyond_a_launch_are_refused():
+    """Fewer than 2^32 threads go into one launch."""
+    L, n = _lib.lib(), ctypes.c_size_t(0)
+    q = L.rnnt_mi355x_beam_select_workspace_bytes
+    for big in ((1 << 22, 1, 8, 4), (1 << 20, 32, 4097, 4), ((1 << 22) - 1, 1, 40000, 4)):
+        assert q(*big, ctypes.byref(n)) == _lib.UNSUPPORTED_SIZE
+    assert q((1 << 22) - 1, 64, 2048, 4, ctypes.byref(n)) == 0 and q((1 << 20) - 1, 32, 4096, 4, ctypes.byref(n)) == 0
+    q = L.rnnt_mi355x_layer_workspace_bytes
+    assert q(_layer(rows=(1 << 30) - 63), None, 0, ctypes.byref(n), None) == _lib.UNSUPPORTED_SIZE
+    assert q(_layer(rows=(1 << 30) - 64), None, 0, ctypes.byref(n), None) == 0
