@@ -20,7 +20,7 @@ def dense(x, kernel, bias=None, activation="linear", residual=None, dropout=0.0,
     "linear", "tanh", "relu", "gelu" (z times the normal distribution's function) or "silu".  dropout, seed, offset: as
     ``rnnt_amd.dropout`` takes them, the mask being the one it draws for the result; rate 0 at inference.
 
-  The same inputs give the same bits, forward and backward.  The gradient is not differentiable itself (create_graph is
+    The same inputs give the same bits, forward and backward.  The gradient is not differentiable itself (create_graph is
     refused)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
