@@ -15,8 +15,8 @@
 //     max(a[i], b[P-1-i]) are the P largest, and log2 P exchanges sort them.
 // Rows of up to 2048 symbols take one launch, a block per utterance; longer ones a launch over pieces of 2048 and one that
 // joins the pieces' lists.  Measured, 32 utterances x 16 beams x 32003 symbols in bfloat16 with a mask: pieces 17.5 us (34 MB;
-// half of it are the 27 instructions a symbol), join 9.8 us; 4 x 32 x 65536 in float16 without one: 11 and 15 us; 64 x 8 x 1024
-// in float32: 8.6 us.  The joins, and the short rows, are chains of latencies: sorting networks over a wavefront, LDS, memory.
+// half of it are the 27 instructions a symbol), join 7.5 us; 4 x 32 x 65536 in float16 without one: 11 and 11 us; 64 x 8 x 1024
+// in float32: 7.5 us.  The joins, and the short rows, are chains of latencies: sorting networks over a wavefront, LDS, memory.
 #include "op_util.h"
 
 namespace {
@@ -401,15 +401,29 @@ __global__ __launch_bounds__(E > 8 ? 512 : 1024) void k_beam_rows(BeamArgs a) {
     }
     join<P>(acc, t, lane);
   }
-  join_block<P>(acc, tree, wave, waves, lane);
+  int active = 1;  // wavefronts that took beams, up to a power of two
+  while (active * G < a.K && active < waves) active <<= 1;
+  join_block<P>(acc, tree, wave, active, lane);
   if (wave == 0) write_out(a, b, lane, acc);
+}
+
+// The block's keys whose lanes say `in`, into LDS in any order; *n counts them, and past 64 they are not kept.
+__device__ __forceinline__ void gather(const TotalKey& k, bool in, int lane, TotalKey* buf, int* n) {
+  const uint64_t who = __ballot(in);
+  if (!who) return;  // uniform
+  int at = 0;
+  if (lane == 0) at = atomicAdd(n, __popcll(who));
+  at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
+  if (in && at < 64) buf[at] = k;
 }
 
 // Long rows, first launch: a wavefront per piece.  Workspace: the pieces' sums, then their lists of P keys.
 struct PieceSum {
   double s;
-  float m, pad;
+  float m;        // the value of the list's first entry, -inf where there is none
+  uint32_t best;  // its `lo`
 };
+__device__ __forceinline__ RowKey head_of(const PieceSum& q) { return q.m > -INFINITY ? RowKey{ordered(q.m + 0.f), q.best} : RowKey{0u, 0u}; }
 template <class T, int P>
 __global__ __launch_bounds__(256) void k_beam_pieces(BeamArgs a, PieceSum* sums, RowKey* lists) {
   __shared__ RowKey buf[4][64];
@@ -424,7 +438,7 @@ __global__ __launch_bounds__(256) void k_beam_pieces(BeamArgs a, PieceSum* sums,
   load_piece<T, kPiece / 64>(a, (int)(row / (unsigned)a.K), (int)(row % (unsigned)a.K), piece * kPiece, lane, x);
   const RowKey best = best_of_piece<kPiece / 64>(x, piece * kPiece, a.width, lane, buf[wave], &m, &s);
   if (lane < P) lists[(long long)id * P + lane] = lane < a.width ? best : RowKey{0u, 0u};
-  if (lane == 0) sums[id] = PieceSum{s, m, 0.f};
+  if (lane == 0) sums[id] = PieceSum{s, m, best.lo};
 }
 
 // Second launch: a block per utterance joins the pieces.  Only the `width` lists with the best first entries can hold
@@ -436,41 +450,80 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
   __shared__ bool over[kMaxBeams];   // finished: its score is its one candidate
   __shared__ TotalKey tree[16][64];
   __shared__ TotalKey best[kMaxWidth];
+  __shared__ uint32_t most[kMaxBeams];  // the largest value of a beam's row
+  __shared__ double terms[64][kMaxBeams];
+  __shared__ uint32_t tops[64];
+  __shared__ TotalKey few[64];
+  __shared__ int found[2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, b = blockIdx.x;
   const int lists_here = a.K * a.pieces;
   lists += (long long)b * lists_here * P;
-  // everything that the first half needs is asked for at once
+  if (threadIdx.x < 2) found[threadIdx.x] = 0;
+  if (threadIdx.x < 64) tops[threadIdx.x] = 0u;
   const int first = wave * 64 + lane;
-  RowKey head = {0u, 0u};
-  if (first < lists_here) head = lists[(long long)first * P];
-  for (int k = wave; k < a.K; k += waves) {
-    const long long row = (long long)b * a.K + k;
-    const PieceSum* mine = sums + row * a.pieces;
-    const float given = a.scores[row];
-    const bool done = a.finished && a.finished[row];
-    PieceSum q = {0.0, -INFINITY, 0.f};
-    if (lane < a.pieces) q = mine[lane];
-    float score = given;
-    RowSum of = {0.0, 0.0};
-    if (!live_score(score)) score = NAN;
-    else if (!done) {  // uniform
-      float m = q.m;
-      for (int p = lane + 64; p < a.pieces; p += 64) m = fmaxf(m, mine[p].m);
-      m = wave_max(m);
-      // a piece without an allowed symbol has m = -inf and s = 0; a NaN sum stays one
-      double s = q.m == -INFINITY ? q.s : q.s * exp((double)q.m - (double)m);
-      for (int p = lane + 64; p < a.pieces; p += 64) {
-        const PieceSum o = mine[p];
-        s += o.m == -INFINITY ? o.s : o.s * exp((double)o.m - (double)m);
-      }
-      s = wave_sum(s);
-      of = RowSum{(double)m, log(s)};
-      if (!(s > 0.0)) score = NAN;
+  sums += (long long)b * lists_here;
+  PieceSum q = {0.0, -INFINITY, 0u};
+  if (first < lists_here) q = sums[first];
+  auto piece = [&](int l) { return l == first ? q : sums[l]; };
+  // a piece without an allowed symbol has m = -inf and s = 0; a NaN sum stays one
+  auto term = [](const PieceSum& q, float m) { return q.m == -INFINITY ? q.s : q.s * exp((double)q.m - (double)m); };
+  auto note = [&](int k, float score, bool done, float m, double s) {
+    if (!live_score(score) || (!done && !(s > 0.0))) score = NAN;
+    rows[k] = RowSum{(double)m, log(s)};
+    live[k] = score;
+    over[k] = done;
+  };
+  if (a.pieces <= 64) {
+    // A thread per piece, then one per beam: a double's exp and log are some hundred instructions, which a wavefront per beam
+    // goes through beam after beam (the join of 32 x 16 x 32003: 10.0 us that way, 8.0 this way).  Longer rows fill wavefronts.
+    auto read = [&](int k) {  // a beam whose pieces were made
+      const long long row = (long long)b * a.K + k;
+      return live_score(a.scores[row]) && !(a.finished && a.finished[row]);
+    };
+    const bool mine = first < lists_here && read(first / a.pieces);
+    float score = NAN;
+    bool done = false;
+    if ((int)threadIdx.x < a.K) {
+      const long long row = (long long)b * a.K + threadIdx.x;
+      score = a.scores[row];
+      done = a.finished && a.finished[row];
     }
-    if (lane == 0) {
-      rows[k] = of;
-      live[k] = score;
-      over[k] = done;
+    if ((int)threadIdx.x < kMaxBeams) most[threadIdx.x] = 0u;
+    __syncthreads();
+    for (int l = first; l < lists_here; l += waves * 64) {
+      const int k = l / a.pieces;
+      if (l == first ? mine : read(k)) atomicMax(&most[k], ordered(piece(l).m));
+    }
+    __syncthreads();
+    for (int l = first; l < lists_here; l += waves * 64) {
+      const int k = l / a.pieces;
+      if (l == first ? mine : read(k)) terms[l - k * a.pieces][k] = term(piece(l), unordered(most[k]));
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.K) {
+      const int k = threadIdx.x;
+      double s = 0.0;
+      if (most[k]) {
+#pragma unroll 8
+        for (int p = 0; p < a.pieces; ++p) s += terms[p][k];
+      }
+      note(k, score, done, unordered(most[k]), s);
+    }
+  } else {
+    for (int k = wave; k < a.K; k += waves) {
+      const long long row = (long long)b * a.K + k;
+      const PieceSum* mine = sums + k * a.pieces;
+      const float score = a.scores[row];
+      const bool done = a.finished && a.finished[row];
+      float m = -INFINITY;
+      double s = 0.0;
+      if (live_score(score) && !done) {  // uniform
+        for (int p = lane; p < a.pieces; p += 64) m = fmaxf(m, mine[p].m);
+        m = wave_max(m);
+        for (int p = lane; p < a.pieces; p += 64) s += term(mine[p], m);
+        s = wave_sum(s);
+      }
+      if (lane == 0) note(k, score, done, m, s);
     }
   }
   __syncthreads();
@@ -481,32 +534,67 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamArgs a, const PieceSum* 
     if (!over[k]) return total_key(a, k, false, score, rows[k], c);
     return r == 0 && l == k * a.pieces ? total_key(a, k, true, score, rows[k], RowKey{0u, 0u}) : TotalKey{0ull, 0u};
   };
+  // As in a piece: of 64 maxima (lists 64 apart, so that every beam has a part in many) the width-th bounds the width-th head
+  // from below, and the few heads that reach it are sorted by one wavefront (the join of 4 x 32 x 65536: 11.0 us, with lists of
+  // 64 sorted and joined across the block 14.7).  Where they are more than 64, that is done still.
   TotalKey heads = {0ull, 0u};
+  if (first < lists_here) heads = entry(first, 0, head_of(q));
+  const TotalKey mine = heads;
+  auto head = [&](int l) { return l >= lists_here ? TotalKey{0ull, 0u} : l == first ? mine : entry(l, 0, head_of(sums[l])); };
+  for (int l = first; l < lists_here; l += waves * 64) atomicMax(&tops[lane], (uint32_t)(head(l).hi >> 32));
+  __syncthreads();
+  uint32_t least = tops[lane];
+  sort64_values(least, lane);
+  least = max(1u, (uint32_t)__shfl((int)least, a.width - 1, 64));
   for (int l = first; l - lane < lists_here; l += waves * 64) {
-    TotalKey t = {0ull, 0u};
-    if (l < lists_here) t = entry(l, 0, l == first ? head : lists[(long long)l * P]);
-    if (__any(t.hi != 0)) {
-      sort64(t, lane);
-      join<64>(heads, lane_xor<63>(t), lane);
-    }
+    const TotalKey t = head(l);
+    gather(t, (uint32_t)(t.hi >> 32) >= least, lane, few, &found[0]);
   }
-  join_block<64>(heads, tree, wave, waves, lane);
+  __syncthreads();
+  if (found[0] <= 64) {
+    if (wave == 0) {
+      heads = lane < found[0] ? few[lane] : TotalKey{0ull, 0u};
+      sort64(heads, lane);
+    }
+  } else {
+    sort64(heads, lane);
+    for (int l = first + waves * 64; l - lane < lists_here; l += waves * 64) {
+      TotalKey t = head(l);
+      if (__any(t.hi != 0)) {
+        sort64(t, lane);
+        join<64>(heads, lane_xor<63>(t), lane);
+      }
+    }
+    join_block<64>(heads, tree, wave, waves, lane);
+  }
   if (wave == 0 && lane < a.width) best[lane] = heads;
   __syncthreads();
 
   TotalKey acc = {0ull, 0u};
   constexpr int G = 64 / P;
   const int i = lane & (P - 1), r = P - 1 - i;
-  for (int l0 = wave * G; l0 < a.width; l0 += waves * G) {
-    TotalKey t = {0ull, 0u};
+  auto kept = [&](int l0) {  // of the lists with the best heads, the l0-th and on, P entries each and the last first
     const int w = l0 + lane / P;
-    if (w < a.width && best[w].hi) {
-      const uint32_t flat = ~best[w].lo, k = flat / (uint32_t)a.V;
-      const int l = (int)k * a.pieces + (over[k] ? 0 : (int)(flat - k * (uint32_t)a.V) / kPiece);
-      t = entry(l, r, over[k] ? RowKey{0u, 0u} : lists[(long long)l * P + r]);
-    }
-    join<P>(acc, t, lane);
+    if (w >= a.width || !best[w].hi) return TotalKey{0ull, 0u};
+    const uint32_t flat = ~best[w].lo, k = flat / (uint32_t)a.V;
+    const int l = (int)k * a.pieces + (over[k] ? 0 : (int)(flat - k * (uint32_t)a.V) / kPiece);
+    return entry(l, r, over[k] ? RowKey{0u, 0u} : lists[(long long)l * P + r]);
+  };
+  // the last of these heads bounds the result, too
+  least = max(1u, (uint32_t)(best[a.width - 1].hi >> 32));
+  for (int l0 = wave * G; l0 < a.width; l0 += waves * G) {
+    const TotalKey t = kept(l0);
+    gather(t, (uint32_t)(t.hi >> 32) >= least, lane, few, &found[1]);
   }
+  __syncthreads();
+  if (found[1] <= 64) {
+    if (wave > 0) return;
+    if (lane < found[1]) acc = few[lane];
+    sort64(acc, lane);
+    write_out(a, b, lane, acc);
+    return;
+  }
+  for (int l0 = wave * G; l0 < a.width; l0 += waves * G) join<P>(acc, kept(l0), lane);
   join_block<P>(acc, tree, wave, waves, lane);
   if (wave == 0) write_out(a, b, lane, acc);
 }

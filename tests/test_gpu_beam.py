@@ -255,3 +255,18 @@ def test_reorder_of_conjugate_and_negated_views():
     for v in (s.conj(), s.conj().imag):
         (got,) = rnnt_amd.beam_reorder(parent, [v])
         assert torch.equal(got, v.resolve_conj().resolve_neg().gather(1, index))
+
+
+@pytest.mark.parametrize("W", [7, 32, 64])
+@pytest.mark.parametrize("spread", [0.5, 40.0])
+def test_lists_of_many_pieces(W, spread):
+    """What the second launch chooses from: beams alike, in order, and one that has everything; equal values everywhere; more lists than
+    a block has lanes; 64 pieces a row and one more; finished and empty beams among them."""
+    for B, K, V, dtype in ((1, 32, 12000, torch.float16), (1, 64, 33000, torch.bfloat16), (1, 3, 131072, torch.float32), (1, 3, 131073, torch.bfloat16)):
+        logits, scores, kw = case(B, K, V, dtype, K + V, finished=K == 3)
+        scores = scores - spread * torch.arange(K)
+        scores[0, K // 2] = float("nan")
+        run(logits, scores, W, kw)
+        if K == 32:
+            run(logits[:, :1].expand(B, K, V).contiguous(), torch.full((B, K), -1.0), W, kw)
+    run(torch.zeros(2, 20, 6000), -spread * torch.arange(40).reshape(2, 20).float(), W, {})
