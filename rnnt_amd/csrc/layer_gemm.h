@@ -233,7 +233,7 @@ struct Tile {
   using E = typename T::elem;
   static constexpr int kPieces = R * BK / 8, kEach = kPieces / THREADS, kRow = KS ? R / 8 : BK / 8;
   static constexpr int kPlaneBytes = R * BK * 2, kBytes = kPlaneBytes * kPlanes<T>;
-  static_assert(kPieces % THREADS == 0 && (!KS || R >= 64) && (BK == 32 || BK == 64), "tile shape");
+  static_assert(kPieces % THREADS == 0 && (!KS || R >= 32) && (BK == 32 || BK == 64), "tile shape");
 
   static_assert((THREADS & (THREADS - 1)) == 0, "");
   static __device__ __forceinline__ int tid() { return threadIdx.x & (THREADS - 1); }  // of the wavefronts that share this tile
@@ -241,7 +241,7 @@ struct Tile {
   // place p holds row p / kRow and piece (p % kRow) ^ permute(row).  64 banks serve 256 bytes a cycle: k-fast reads take one
   // piece of 16 rows together, k-slow reads 64 bytes of 4 consecutive k.
   static __device__ __forceinline__ int permute(int row) {
-    if constexpr (KS) return kRow == 8 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+    if constexpr (KS) return kRow == 4 ? 0 : kRow == 8 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
     else return kRow == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
   }
 

@@ -30,6 +30,9 @@ int launch_block(int block, const GemmArgs& g, hipStream_t st) {
     case kBlock64Groups:
       if constexpr (PRODUCT != kKernelGrad) return launch_gemm<T, PRODUCT, 64, 64, BK, 32, 32, DIRECT, 4>(g, st);
       break;
+    case kBlock64Thin:
+      if constexpr (PRODUCT == kForward && DIRECT) return launch_gemm<T, PRODUCT, 64, 32, 32, 32, 32, DIRECT, 4>(g, st);
+      break;
     case kBlock128x128: return launch_gemm<T, PRODUCT, 128, 128, BK, 64, 64, DIRECT>(g, st);
     case kBlock256x256:
       if constexpr (DIRECT) return launch_gemm<T, PRODUCT, 256, 256, 64, 128, 64, DIRECT>(g, st);

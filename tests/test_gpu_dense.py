@@ -330,3 +330,9 @@ def test_activations_of_small_numbers_are_relative(dtype, act, rows):
     want = orc.activation(f64(z), act)[0][:, None]
     tol = (2.0 ** -18 + U[dtype] * 1.01) * np.abs(want) + 2 * LEAST[dtype] + 2.0 ** -125
     assert (np.abs(f64(y) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(33, 2048, 2000), (64, 8, 2048), (50, 1992, 4104), (64, 2048, 8192), (64, 2056, 8192)])
+def test_some_rows_of_a_wide_layer(M, K, N, dtype):
+    check_layer(M, K, N, dtype, "silu", True, True, 0.2)
