@@ -1,5 +1,5 @@
 """Plain float64 numpy forms of the operators around the joint network: the counter-based dropout mask, Dense with its
-epilogue, the beam step.  A checker, like everything in this folder."""
+epilogue, the beam step.  An oracle, like everything in this folder."""
 import math
 
 import numpy as np

@@ -1,4 +1,4 @@
-"""The beam step against the float64 checker.  Places (parents, tokens) have to be equal; a total is a float64 sum rounded to
+"""The beam step against the float64 oracle.  Places (parents, tokens) have to be equal; a total is a float64 sum rounded to
 float32, whose log sum exp comes from float32 exponentials good to 2 units in the last place (2^-22 relative, so 2^-22 absolute in the
 logarithm): tolerance 2^-24 |total| + 2^-22."""
 import numpy as np

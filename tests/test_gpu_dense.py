@@ -1,4 +1,4 @@
-"""Dense layer with its epilogue against the float64 checker.
+"""Dense layer with its epilogue against the float64 oracle.
 
 Tolerances, with u = half a step of the type (fp32 2^-24, bf16 2^-8, fp16 2^-11; float16 below 2^-14: 2^-25 absolute):
   product       a float32 accumulation of K products: each of at most K + 3 roundings is 2^-24 of a partial sum, which is

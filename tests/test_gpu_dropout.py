@@ -1,4 +1,4 @@
-"""Dropout with a mask that is never stored, against the float64 checker.  y = x * c with c = 1/keep in float32: the scale and
+"""Dropout with a mask that is never stored, against the float64 oracle.  y = x * c with c = 1/keep in float32: the scale and
 the product are each rounded to float32, and 16-bit types round once more; a tolerance counts half a step for each."""
 import numpy as np
 import pytest

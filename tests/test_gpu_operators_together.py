@@ -1,5 +1,5 @@
 """The operators as they are used together: a training step of the fully-connected joint with dropout against float64, and a
-decoder's steps (dense on the beam's rows, selection, states in their new order) against the float64 checker."""
+decoder's steps (dense on the beam's rows, selection, states in their new order) against the float64 oracle."""
 import gc
 
 import numpy as np
@@ -71,7 +71,7 @@ def test_an_offset_in_device_memory_gives_the_same_step():
 @pytest.mark.parametrize("V", [62, 2500])
 def test_decoder_steps(V, dtype):
     """Three steps of a beam search over a small recurrent prediction network: hidden layer with a skip connection, output layer,
-    selection, reordering.  The checker selects from the very logits the layers gave, in float64."""
+    selection, reordering.  The oracle selects from the very logits the layers gave, in float64."""
     g = torch.Generator().manual_seed(4)
     B, K, H = 3, 4, 48
     def t(*s, scale=1.0):

@@ -1,4 +1,4 @@
-"""Dropout and beam operators without a GPU: known answers of the generator's checker, refusals of the C entry points before
+"""Dropout and beam operators without a GPU: known answers of the generator's oracle, refusals of the C entry points before
 any launch, refusals of the Python entry points."""
 import ctypes
 
@@ -133,7 +133,7 @@ def test_rates_and_seeds():
     assert _operator.seed_offset("d", 3, t, cpu) == (3, 0, t)
 
 
-def test_checker_of_the_mask_keeps_the_right_share():
+def test_oracle_of_the_mask_keeps_the_right_share():
     s = orc.dropout_scale(400, 501, 0.3, 5, 9)
     n = s.size
     kept = (s > 0).sum()
