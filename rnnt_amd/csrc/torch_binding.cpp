@@ -361,6 +361,16 @@ std::pair<uintptr_t, uintptr_t> bytes_of(const Tensor& t) {
   return {p, p + (uintptr_t)((last + 1) * t.element_size())};
 }
 
+// A state as [outer, B, K, row], its row dense: outer, and the strides of the three leading dimensions in elements.  A dense
+// tensor's come from its sizes: where a dimension has size 1 its own stride may be anything.
+std::tuple<int64_t, int64_t, int64_t, int64_t> leading(const Tensor& s, int64_t d) {
+  int64_t outer = 1, row = 1;
+  for (int64_t j = 0; j < d; ++j) outer *= s.size(j);
+  if (!s.is_contiguous()) return {outer, d ? s.stride(d - 1) : 0, s.stride(d), s.stride(d + 1)};
+  for (int64_t j = d + 2; j < s.dim(); ++j) row *= s.size(j);
+  return {outer, s.size(d) * s.size(d + 1) * row, s.size(d + 1) * row, row};
+}
+
 std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<Tensor>& states, int64_t d, const std::optional<std::vector<Tensor>>& out_given) {
   const char* op = "beam_reorder";
   if (parent_given.scalar_type() != at::kInt || parent_given.dim() != 2) bad_value("beam_reorder: parent must be int32 [B, W]");
@@ -428,10 +438,9 @@ std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<T
       if (!dense_row) s = s.contiguous();
       keep.push_back(s);
     }
+    const auto [outer, outer_stride, batch_stride, beam_stride] = leading(s, d);
     const int64_t e = s.element_size();
-    int64_t outer = 1;
-    for (int64_t j = 0; j < d; ++j) outer *= s.size(j);
-    table.push_back({s.data_ptr(), o.data_ptr(), outer, d ? s.stride(d - 1) * e : 0, s.stride(d) * e, s.stride(d + 1) * e, o.numel() / (outer * B * W) * e});
+    table.push_back({s.data_ptr(), o.data_ptr(), outer, outer_stride * e, batch_stride * e, beam_stride * e, o.numel() / (outer * B * W) * e});
   }
   for (size_t i = 0; i < table.size(); i += RNNT_MI355X_REORDER_MAX)
     check(C.beam_reorder(table.data() + i, (int)std::min<size_t>(RNNT_MI355X_REORDER_MAX, table.size() - i), parent.data_ptr<int32_t>(), (int)B, (int)K, (int)W,
@@ -448,4 +457,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("dense", &dense);
   m.def("beam_select", &beam_select);
   m.def("beam_reorder", &beam_reorder);
+  m.def("reorder_strides", &leading);  // of beam_reorder, for tests without a GPU
 }

@@ -270,3 +270,16 @@ def test_lists_of_many_pieces(W, spread):
         if K == 32:
             run(logits[:, :1].expand(B, K, V).contiguous(), torch.full((B, K), -1.0), W, kw)
     run(torch.zeros(2, 20, 6000), -spread * torch.arange(40).reshape(2, 20).float(), W, {})
+
+
+def test_reorder_of_a_state_with_a_dimension_of_size_one():
+    """[layers, 1, B, K, hidden] made by transposing [1, layers, ...]: dense, though the stride of its dimension of size 1 is not the
+    distance of the layers."""
+    base = torch.randn(1, 3, 2, 4, 5, generator=torch.Generator().manual_seed(13)).to(DEV)
+    s = base.transpose(0, 1)
+    assert s.is_contiguous() and s.stride(1) != s.stride(0)
+    parent = torch.tensor([[2, 0, 3], [-1, 1, 1]], dtype=torch.int32, device=DEV)
+    (got,) = rnnt_amd.beam_reorder(parent, [s], batch_dim=2)
+    want = s[:, :, torch.arange(2, device=DEV)[:, None], parent.clamp(min=0).long()]
+    want[:, :, 1, 0] = 0
+    assert torch.equal(got, want)

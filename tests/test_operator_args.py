@@ -158,3 +158,14 @@ def test_calls_beyond_a_launch_are_refused():
     q = L.rnnt_mi355x_layer_workspace_bytes
     assert q(_layer(rows=(1 << 30) - 63), None, 0, ctypes.byref(n), None) == _lib.UNSUPPORTED_SIZE
     assert q(_layer(rows=(1 << 30) - 64), None, 0, ctypes.byref(n), None) == 0
+
+
+def test_strides_of_a_dense_state_come_from_its_sizes():
+    """A dimension of size 1 may carry any stride in a tensor that is dense all the same."""
+    strides = _lib.native().reorder_strides
+    s = torch.empty(1, 3, 2, 5, 4).transpose(0, 1)  # [3, 1, B, K, 4]
+    assert s.is_contiguous() and s.stride(1) == 3 * 40
+    assert strides(s, 2) == (3, 40, 20, 4)
+    assert strides(torch.empty(2, 5, 4).as_strided((1, 2, 5, 4), (7, 20, 4, 1)), 1) == (1, 40, 20, 4)
+    assert strides(torch.empty(6, 2, 5, 4)[::2], 1) == (3, 80, 20, 4)
+    assert strides(torch.empty(2, 5), 0) == (1, 10, 5, 1)
