@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <unordered_set>
+
 #include "../../include/rnnt_mi355x.h"
 
 namespace py = pybind11;
@@ -76,23 +78,31 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
-// Where a backward pass is captured, autograd makes the stream of every node behind this one wait for the stream captured.  A
+// Where a backward pass is captured, autograd makes the stream of every node that it comes to wait for the stream captured.  A
 // leaf that an eager graph still uses has its node on that graph's stream, and such a wait from outside the capture ends the
-// process; it is refused before it happens.
+// process; it is refused before it happens, wherever behind the operator's node that leaf is.  (What does not lie behind an
+// operator's node is not seen from here.)
 void refuse_waits_outside_capture(const char* op) {
   const auto here = c10::hip::getCurrentHIPStream();
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  const auto node = torch::autograd::get_current_node();
-  for (uint32_t i = 0; node && i < node->num_outputs(); ++i) {
-    const auto& next = node->next_edge(i).function;
-    if (!next || !node->task_should_compute_output(i)) continue;
-    const auto there = next->stream();
-    if (!there || (there->id() == here.id() && there->device_index() == here.device_index())) continue;
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *there).stream();
-    const bool captured = other && hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
-    TORCH_CHECK(captured, op, ": this backward pass is being captured, and goes on to a tensor that an eager graph on another stream still holds; "
-                          "drop that graph and its results first, or give the captured pass leaves of its own");
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  if (const auto node = torch::autograd::get_current_node()) todo.push_back(node.get());
+  while (!todo.empty()) {
+    torch::autograd::Node* const node = todo.back();
+    todo.pop_back();
+    for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+      const auto& next = node->next_edge(i).function;
+      if (!next || !node->task_should_compute_output(i) || !seen.insert(next.get()).second) continue;
+      todo.push_back(next.get());
+      const auto there = next->stream();
+      if (!there || (there->id() == here.id() && there->device_index() == here.device_index())) continue;
+      hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+      const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *there).stream();
+      const bool captured = other && hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+      TORCH_CHECK(captured, op, ": this backward pass is being captured, and goes on to a tensor that an eager graph on another stream still holds; "
+                            "drop that graph and its results first, or give the captured pass leaves of its own");
+    }
   }
 }
 

@@ -129,3 +129,32 @@ def test_captured_backward_pass_of_leaves_that_an_eager_graph_holds_is_refused()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, step(w)))
     assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+@pytest.mark.parametrize("op", ["dense", "dropout"])
+def test_captured_backward_pass_is_refused_where_the_leaf_lies_behind_other_nodes(op):
+    """The leaf that the eager graph holds comes several nodes behind the operator's own."""
+    x = torch.randn(30, 20, device=DEV)
+    w = (torch.randn(20, 16, device=DEV) * 0.2).requires_grad_(True)
+
+    def layer(w):
+        k = (w * 1.5).tanh().t().contiguous().t()
+        return rnnt_amd.dense(x, k, None, "silu") if op == "dense" else rnnt_amd.dropout(k, 0.25, seed=3)
+
+    def step(w):
+        y = layer(w)
+        return torch.autograd.grad((y * y).sum(), w)
+    eager = w.sin()
+    with pytest.raises(RuntimeError, match="eager graph on another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step(w)
+    del eager
+    gc.collect()
+    (want,) = step(w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        (out,) = step(w)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
