@@ -17,7 +17,8 @@ def dense(x, kernel, bias=None, activation="linear", residual=None, dropout=0.0,
 
     x [..., in], kernel [in, out] (Keras layout), bias [out], residual [..., out]: one of float32, bfloat16, float16, the same
     for all; the result has that type, products and sums are float32 throughout (float32 inputs included).  activation:
-    "linear", "tanh", "relu", "gelu" (z times the normal distribution's function) or "silu".  dropout, seed, offset: as
+    "linear", "tanh", "relu", "gelu" (z times the normal distribution's function, its error relative to the
+    result also in the negative tail) or "silu".  dropout, seed, offset: as
     ``rnnt_amd.dropout`` takes them, the mask being the one it draws for the result; rate 0 at inference.
 
     The same inputs give the same bits, forward and backward.  The gradient is not differentiable itself (create_graph is

@@ -12,6 +12,8 @@ Tolerances, with u = half a step of the type (fp32 2^-24, bf16 2^-8, fp16 2^-11;
                 a float32 one has the product's own error) and one rounding u to the type; dx, dkernel, dbias then are sums
                 of such terms: the same bound with S over |dz||w| plus the sum of the terms' errors.
 """
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -336,3 +338,30 @@ def test_activations_of_small_numbers_are_relative(dtype, act, rows):
 @pytest.mark.parametrize("M,K,N", [(33, 2048, 2000), (64, 8, 2048), (50, 1992, 4104), (64, 2048, 8192), (64, 2056, 8192)])
 def test_some_rows_of_a_wide_layer(M, K, N, dtype):
     check_layer(M, K, N, dtype, "silu", True, True, 0.2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [8, 600])
+def test_gelu_keeps_its_digits_in_the_negative_tail(dtype, rows):
+    """z Phi(z) between -12.5 and -1, relative to itself.  With a kernel of one, z is x: exact in 16 bits; the three parts of a float32
+    are each summed once, 4 x 2^-24 of z at most, which the tail, exp(-z^2/2), takes z^2 times.
+    float32: e^(-z^2/2) has an argument off by 2.5 x 2^-24 of itself: 1.25 z^2 2^-24; the fit 2 x 2^-24, reciprocal, polynomial, exp2 and
+    the products 20 roundings or less.  16 bits: 2^-13 by the fit where float16 results are not zero, 2^-9.8 further out; half a step of
+    the type."""
+    z = torch.linspace(-12.5, -1.0, rows, dtype=torch.float64).to(dtype)
+    x = z.to(DEV)[:, None].requires_grad_(True)
+    y = rnnt_amd.dense(x, torch.ones(1, 5, dtype=dtype, device=DEV), None, "gelu")
+    f = f64(z)
+    phi = np.array([0.5 * math.erfc(-v / math.sqrt(2.0)) for v in f])
+    want = (f * phi)[:, None]
+    rel = (5.25 * f * f + 24) * 2.0 ** -24 if dtype == torch.float32 else np.where(f > -5.9, 2.0 ** -13, 2.0 ** -9.8) + U[dtype] * 1.01
+    assert (np.abs(f64(y) - want) <= rel[:, None] * np.abs(want) + LEAST[dtype]).all()
+    if dtype == torch.bfloat16:
+        return  # its slope comes from a float16 pre-activation
+    # Phi(z) + z phi(z): from z = -1.2 on the two terms' sizes add up to 3 times their sum's at most; dz is rounded to the type, the gradient
+    # is one column of it times a kernel of one, rounded again
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y) * torch.tensor([1.0, 0, 0, 0, 0], dtype=dtype, device=DEV))
+    slope = phi + f * np.exp(-f * f / 2) / math.sqrt(2 * math.pi)
+    rel = (5.25 * f * f + 24) * 3 * 2.0 ** -24 + (0 if dtype == torch.float32 else U[dtype] * 2.02)
+    far = f <= -1.2
+    assert (np.abs(f64(dx)[:, 0] - slope) <= rel * np.abs(slope) + 2 * LEAST[dtype])[far].all()
