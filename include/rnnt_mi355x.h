@@ -306,7 +306,7 @@ int rnnt_mi355x_layer_backward(const rnnt_mi355x_layer* layer, const void* dy, l
  * [B, V] or NULL, zero forbids a symbol (its logit is not looked at and has no part in
  * the softmax; allowed_batch_stride 0: one mask for all utterances); finished: bytes
  * [B, K] or NULL: such a beam offers itself alone, with its score, at symbol `end`.
- *   total = scores + x - log sum exp x          (ordered in float64)
+ *   total = scores + x - log sum exp x          (ordered in float64; the logarithm is off by at most 2^-21.6)
  * and the `width` largest totals of an utterance, ties to the lowest k*V + v, go to
  * out_scores / out_parent / out_token [B, width]; places without a candidate hold
  * -inf, -1, -1.  A beam whose score is NaN or beyond +-2^30 is empty; so is one whose

@@ -21,7 +21,8 @@ def beam_select(logits, scores, width, enc=None, allowed=None, finished=None, en
     a transducer: a hypothesis that has emitted blank and waits for the next frame).  Nothing is differentiable here.
 
     Returns scores [B, width] float32, parent [B, width] int32 (beam) and token [B, width] int32, in descending order of
-    scores + log_softmax (compared in float64), ties to the lowest beam, then the lowest symbol.  Where there are fewer
+    scores + log_softmax (compared in float64, where a row's log sum exp is good to 2^-21.6: its terms are float32), ties to the lowest
+    beam, then the lowest symbol.  Where there are fewer
     candidates than `width`: -inf, -1, -1.  A beam whose allowed logits hold NaN or +inf, or nothing above -inf, has none."""
     return _lib.native().beam_select(logits, scores, width, enc, allowed, finished, end)
 

@@ -14,14 +14,14 @@
 //   - sorted lists are joined by the first step of a bitonic merge: of two sorted lists a, b the values
 //     max(a[i], b[P-1-i]) are the P largest, and log2 P exchanges sort them.
 // Rows of up to 2048 symbols take one launch, a block per utterance; longer ones a launch over pieces of 2048 and one that
-// joins the pieces' lists.  Measured, 32 utterances x 16 beams x 32003 symbols in bfloat16 with a mask: pieces 17.5 us (34 MB;
-// half of it are the 27 instructions a symbol), join 7.5 us; 4 x 32 x 65536 in float16 without one: 11 and 11 us; 64 x 8 x 1024
-// in float32: 7.5 us.  The joins, and the short rows, are chains of latencies: sorting networks over a wavefront, LDS, memory.
+// joins the pieces' lists.  Measured, 32 utterances x 16 beams x 32003 symbols in bfloat16 with a mask: pieces 19.6 us (34 MB;
+// more than half of it are the 30 instructions a symbol, four of them in float64), join 7.8 us; 4 x 32 x 65536 in float16 without one: 12.1 and
+// 11 us; 64 x 8 x 1024 in float32: 7.9 us.  The joins, and the short rows, are chains of latencies: sorting networks over a wavefront, LDS, memory.
 #include "op_util.h"
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e64 = 1.4426950408889634;
 constexpr float kScoreLimit = 1073741824.f;  // 2^30: a score beyond it marks an empty beam (or is no score at all)
 constexpr int kMaxBeams = 64, kMaxWidth = 64;
 constexpr int kPiece = 2048;  // symbols of a row that one wavefront takes
@@ -125,13 +125,14 @@ __device__ __forceinline__ double lane_xor(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
   return __builtin_bit_cast(double, ((uint64_t)lane_xor<M>((uint32_t)(b >> 32)) << 32) | lane_xor<M>((uint32_t)b));
 }
+__device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN stays
 __device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, lane_xor<1>(v));
-  v = fmaxf(v, lane_xor<2>(v));
-  v = fmaxf(v, lane_xor<7>(v));
-  v = fmaxf(v, lane_xor<15>(v));
-  v = fmaxf(v, lane_xor<16>(v));
-  return fmaxf(v, lane_xor<32>(v));
+  v = largest(v, lane_xor<1>(v));
+  v = largest(v, lane_xor<2>(v));
+  v = largest(v, lane_xor<7>(v));
+  v = largest(v, lane_xor<15>(v));
+  v = largest(v, lane_xor<16>(v));
+  return largest(v, lane_xor<32>(v));
 }
 // the same order of additions in every wavefront: equal rows get equal sums
 __device__ __forceinline__ double wave_sum(double v) {
@@ -254,21 +255,35 @@ template <int E>
 __device__ __forceinline__ RowKey best_of_piece(const float (&x)[E], int v0, int width, int lane, RowKey* buf, float* m, double* s) {
   float top = x[0];
 #pragma unroll
-  for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);  // drops NaN, which the sum keeps
-  if (top != top) top = -INFINITY;
-  const float mx = wave_max(top), base = mx == -INFINITY ? 0.f : mx;
-  // Eight float32 terms pairwise, then float64: the sum decides between candidates of different beams.  A term is off by
-  // about 2^-23 of itself, at random; over a row that leaves some 10^-8 of the sum.
+  for (int e = 1; e < E; ++e) top = largest(top, x[e]);
+  const float mx = wave_max(top);
+  const bool number = mx < INFINITY;
+  // exp(x - mx) = 2^(n + f): the argument in float64 (in float32 its rounding alone would cost 2^-21 of a term ten below the
+  // largest, the same way for all symbols of equal value), as a fixed-point number with 32 bits of fraction by adding 1.5 x 2^20, f
+  // rounded to 23 bits as the significand of 1 + f, and n added to the result's exponent.  A term is off by 2^-24 (1.43 for exp2,
+  // measured over all its arguments, and ln 2 for f); at x = mx it is exact, so that a row of one symbol sums to 1.  Terms
+  // below 2^-120 become that.  Eight terms are added pairwise in float32, another 3 x 2^-24 where their bits differ, then in
+  // float64: the sum decides between candidates of different beams.  The same with the argument in float32 and a first-order
+  // correction for what it leaves out: 32 x 16 x 32003 in bfloat16 31.0 us a step (29.7 this way, 27.6 without any).
+  const double base = mx == -INFINITY || !number ? 0.0 : (double)mx;
+  constexpr double kFixed = 1572864.0 + 0x1p-24, kLeast = kFixed - 120.0;
   double sum = 0.0;
 #pragma unroll
   for (int e = 0; e < E; e += 8) {
     float t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f((x[e + i] - base) * kLog2e);  // 2^-inf = 0
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t h = __builtin_bit_cast(uint64_t, fmax(fma((double)x[e + i] - base, kLog2e64, kFixed), kLeast));
+      const float f = __uint_as_float(__builtin_amdgcn_alignbit(0x7fu, (uint32_t)h, 9));  // 1 <= f < 2: terms are doubled
+      uint32_t n = (uint32_t)(h >> 32);
+      asm("" : "+v"(n));  // else three instructions take the place of the shift and add that the next line is
+      t[i] = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(f)) + (n << 23));
+    }
     sum += (double)(((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
   }
-  *m = mx;
-  *s = wave_sum(sum);
+  sum = wave_sum(sum);
+  *m = number ? mx : 0.f;
+  *s = !number ? NAN : mx == -INFINITY ? 0.0 : 0.5 * sum;
 
   // `width` lanes have a value of floor_x or more
   uint32_t tops = top > -INFINITY ? ordered(top + 0.f) : 0u;

@@ -283,3 +283,33 @@ def test_reorder_of_a_state_with_a_dimension_of_size_one():
     want = s[:, :, torch.arange(2, device=DEV)[:, None], parent.clamp(min=0).long()]
     want[:, :, 1, 0] = 0
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("V", [2048, 1024, 6 * 2048])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_flat_tails(V, dtype):
+    """One peak over 1023 or 2047 symbols of one value, whose terms are all off by the same amount: nothing averages out.  The sum's error
+    is that of a term, 2^-24 (1.43 + ln 2) for exp2 and its argument, below 2^-22, on top of half a step of the total."""
+    g = torch.Generator().manual_seed(14)
+    n = 60
+    tail = torch.randn(n, generator=g) * 10.0 ** (torch.rand(n, generator=g) * 6 - 5)
+    peak = tail + 5 + 11 * torch.rand(n, generator=g)
+    logits = tail.to(dtype)[:, None].expand(n, V).clone()
+    logits[:, 77::2048] = peak.to(dtype)[:, None]  # long rows are summed in pieces of 2048: a peak in each
+    run(logits.reshape(4, 15, V), -torch.rand(4, 15, generator=g) * 1e-3, 15, {})
+
+
+@pytest.mark.parametrize("pieces", [1, 3])
+def test_beams_whose_totals_are_nearly_the_same(pieces):
+    """Two beams whose best totals are 5e-7 apart, over flat tails of different depth.  The logarithm of a row's sum is good to
+    2.12 x 2^-24 (a term's error), twice that is 2.6e-7."""
+    rows = [(5.9910145, 0.27237773), (5.874392, 0.15194488)]
+    V = 2048 * pieces
+    logits = torch.empty(1, 2, V)
+    for k, (peak, tail) in enumerate(rows):
+        logits[0, k] = tail
+        logits[0, k, 5::2048] = peak
+    x = logits.double()
+    lse = torch.logsumexp(x - x.amax(2, keepdim=True), 2)[0]
+    for gap in (5e-7, -5e-7):
+        run(logits, torch.tensor([[(lse[0] - lse[1] + gap).item(), 0.0]]), 2, {})
