@@ -78,6 +78,15 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+// Results are filled through raw pointers, past everything of torch that follows a computation; what would come out wrong without
+// a word is refused.  A dual tensor of forward-mode differentiation would lose its tangent.
+void refuse_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op, ": forward-mode differentiation is not implemented");
+}
+void refuse_tangents(const char* op, std::initializer_list<const Tensor*> given) {
+  for (const Tensor* t : given) refuse_tangent(op, *t);
+}
+
 // Where a backward pass is captured, autograd makes the stream of every node that it comes to wait for the stream captured.  A
 // leaf that an eager graph still uses has its node on that graph's stream, and such a wait from outside the capture ends the
 // process; it is refused before it happens, wherever behind the operator's node that leaf is.  (What does not lie behind an
@@ -152,6 +161,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
 };
 
 Tensor dropout(const Tensor& x, int64_t drop16, uint64_t seed, uint64_t offset, const OptTensor& offset_t) {
+  refuse_tangent("dropout", x);
   on_gpu("dropout", "x", x);
   code_of("dropout", x);
   if (drop16 == 0 || x.numel() == 0) return x;
@@ -285,6 +295,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
 Tensor dense(const Tensor& x, const Tensor& kernel, const OptTensor& bias_, const OptTensor& residual_, int64_t act, int64_t drop16, uint64_t seed,
              uint64_t offset, const OptTensor& offset_t) {
   const Tensor bias = or_none(bias_), residual = or_none(residual_);
+  refuse_tangents("dense", {&x, &kernel, &bias, &residual});
   on_gpu("dense", "x", x);
   same_device("dense", "kernel", kernel, x);
   same_device("dense", "bias", bias, x);
@@ -317,6 +328,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits_given, const
                                                const OptTensor& allowed_, const OptTensor& finished_, int64_t end) {
   const char* op = "beam_select";
   Tensor logits = logits_given, scores = scores_given, enc = or_none(enc_), allowed = or_none(allowed_), finished = or_none(finished_);
+  refuse_tangents(op, {&logits, &scores, &enc});
   on_gpu(op, "logits", logits);
   same_device(op, "scores", scores, logits);
   same_device(op, "enc", enc, logits);
@@ -383,6 +395,9 @@ std::tuple<int64_t, int64_t, int64_t, int64_t> leading(const Tensor& s, int64_t 
 
 std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<Tensor>& states, int64_t d, const std::optional<std::vector<Tensor>>& out_given) {
   const char* op = "beam_reorder";
+  for (const Tensor& s : states) refuse_tangent(op, s);
+  if (out_given)
+    for (const Tensor& o : *out_given) refuse_tangent(op, o);
   if (parent_given.scalar_type() != at::kInt || parent_given.dim() != 2) bad_value("beam_reorder: parent must be int32 [B, W]");
   on_gpu(op, "parent", parent_given);
   if (d < 0) bad_value("beam_reorder: batch_dim counts from the first dimension");

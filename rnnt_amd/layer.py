@@ -22,7 +22,7 @@ def dense(x, kernel, bias=None, activation="linear", residual=None, dropout=0.0,
     ``rnnt_amd.dropout`` takes them, the mask being the one it draws for the result; rate 0 at inference.
 
     The same inputs give the same bits, forward and backward.  The gradient is not differentiable itself (create_graph is
-    refused)."""
+    refused), and forward-mode differentiation is refused."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"dense: activation must be one of {', '.join(ACTIVATIONS)}")

@@ -18,7 +18,8 @@ def dropout(x, rate, seed=0, offset=0):
 
     x: float32, bfloat16 or float16, any shape.  seed: an integer below 2^64.  offset: an integer below 2^64, or one int64
     on the device (read by the kernel: inside a captured graph the caller advances it between replays); calls that need
-    independent masks take different offsets.  rate 0 returns x itself."""
+    independent masks take different offsets.  rate 0 returns x itself.  Differentiable any number of times, backward; forward-mode
+    differentiation is refused."""
     native = _lib.native()
     if not isinstance(x, torch.Tensor):
         raise TypeError("dropout: x must be a tensor")

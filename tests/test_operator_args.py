@@ -169,3 +169,29 @@ def test_strides_of_a_dense_state_come_from_its_sizes():
     assert strides(torch.empty(2, 5, 4).as_strided((1, 2, 5, 4), (7, 20, 4, 1)), 1) == (1, 40, 20, 4)
     assert strides(torch.empty(6, 2, 5, 4)[::2], 1) == (3, 80, 20, 4)
     assert strides(torch.empty(2, 5), 0) == (1, 10, 5, 1)
+
+
+def _calls(wrap):
+    """Each operator with `wrap` around one of its floating inputs at a time."""
+    x, k, b, r = torch.randn(4, 8), torch.randn(8, 6), torch.randn(6), torch.randn(4, 6)
+    logits, scores, enc = torch.randn(2, 3, 8), torch.zeros(2, 3), torch.randn(2, 8)
+    parent = torch.zeros(2, 3, dtype=torch.int32)
+    yield lambda: rnnt_amd.dense(wrap(x), k, b, residual=r)
+    yield lambda: rnnt_amd.dense(x, wrap(k), b, residual=r)
+    yield lambda: rnnt_amd.dense(x, k, wrap(b), residual=r)
+    yield lambda: rnnt_amd.dense(x, k, b, residual=wrap(r))
+    yield lambda: rnnt_amd.dropout(wrap(x), 0.5)
+    yield lambda: rnnt_amd.beam_select(wrap(logits), scores, 2, enc)
+    yield lambda: rnnt_amd.beam_select(logits, wrap(scores), 2, enc)
+    yield lambda: rnnt_amd.beam_select(logits, scores, 2, wrap(enc))
+    yield lambda: rnnt_amd.beam_reorder(parent, [logits, wrap(logits)])
+    yield lambda: rnnt_amd.beam_reorder(parent, [logits], out=[wrap(torch.zeros(2, 3, 8))])
+
+
+def test_forward_mode_differentiation_is_refused():
+    """A dual tensor does not say requires_grad; its tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        for call in _calls(lambda t: fwd.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
