@@ -5,10 +5,12 @@
 // 6151 x 515 x 1030 in float16 139 and 87.  The entry points are those of the library that rnnt_amd._lib has loaded; their addresses come from there.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <unordered_set>
@@ -80,6 +82,11 @@ Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 // Results are filled through raw pointers, past everything of torch that follows a computation; what would come out wrong without
 // a word is refused.  A dual tensor of forward-mode differentiation would lose its tangent.
+// A trace would hold the allocation of the results and nothing of what is written to them.
+void refuse_tracing(const char* op) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), op,
+              ": calls cannot be traced; trace what is around them");
+}
 void refuse_tangent(const char* op, const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op, ": forward-mode differentiation is not implemented");
 }
@@ -161,6 +168,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
 };
 
 Tensor dropout(const Tensor& x, int64_t drop16, uint64_t seed, uint64_t offset, const OptTensor& offset_t) {
+  refuse_tracing("dropout");
   refuse_tangent("dropout", x);
   on_gpu("dropout", "x", x);
   code_of("dropout", x);
@@ -295,6 +303,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
 Tensor dense(const Tensor& x, const Tensor& kernel, const OptTensor& bias_, const OptTensor& residual_, int64_t act, int64_t drop16, uint64_t seed,
              uint64_t offset, const OptTensor& offset_t) {
   const Tensor bias = or_none(bias_), residual = or_none(residual_);
+  refuse_tracing("dense");
   refuse_tangents("dense", {&x, &kernel, &bias, &residual});
   on_gpu("dense", "x", x);
   same_device("dense", "kernel", kernel, x);
@@ -328,6 +337,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits_given, const
                                                const OptTensor& allowed_, const OptTensor& finished_, int64_t end) {
   const char* op = "beam_select";
   Tensor logits = logits_given, scores = scores_given, enc = or_none(enc_), allowed = or_none(allowed_), finished = or_none(finished_);
+  refuse_tracing(op);
   refuse_tangents(op, {&logits, &scores, &enc});
   on_gpu(op, "logits", logits);
   same_device(op, "scores", scores, logits);
@@ -395,6 +405,7 @@ std::tuple<int64_t, int64_t, int64_t, int64_t> leading(const Tensor& s, int64_t 
 
 std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<Tensor>& states, int64_t d, const std::optional<std::vector<Tensor>>& out_given) {
   const char* op = "beam_reorder";
+  refuse_tracing(op);
   for (const Tensor& s : states) refuse_tangent(op, s);
   if (out_given)
     for (const Tensor& o : *out_given) refuse_tangent(op, o);

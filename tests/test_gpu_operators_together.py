@@ -158,3 +158,20 @@ def test_captured_backward_pass_is_refused_where_the_leaf_lies_behind_other_node
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_tensors_without_memory_of_their_own_never_reach_a_kernel(i):
+    """Transformed, fake and meta tensors have no data pointer: the calls raise."""
+    from torch._subclasses import FakeTensorMode
+    parent, k, scores = torch.zeros(2, 3, dtype=torch.int32, device=DEV), torch.ones(8, 6, device=DEV), torch.zeros(2, 3, device=DEV)
+    call = (lambda x: rnnt_amd.dense(x, k), lambda x: rnnt_amd.dropout(x, 0.5), lambda x: rnnt_amd.beam_select(x, scores, 2)[0],
+            lambda x: rnnt_amd.beam_reorder(parent, [x])[0])[i]
+    x = torch.randn(2, 3, 8, device=DEV)
+    call(x)
+    for bad in (lambda: torch.vmap(call)(x[None]), lambda: torch.func.grad(lambda t: call(t).sum())(x), lambda: call(x.to("meta"))):
+        with pytest.raises((RuntimeError, ValueError)):
+            bad()
+    with FakeTensorMode(), pytest.raises((RuntimeError, ValueError)):
+        call(torch.empty(2, 3, 8, device=DEV))
+    torch.cuda.synchronize()

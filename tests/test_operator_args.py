@@ -195,3 +195,20 @@ def test_forward_mode_differentiation_is_refused():
         for call in _calls(lambda t: fwd.make_dual(t, torch.ones_like(t))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def _operators():
+    parent = torch.zeros(2, 3, dtype=torch.int32)
+    return (lambda x: rnnt_amd.dense(x, torch.ones(8, 6)), lambda x: rnnt_amd.dropout(x, 0.5),
+            lambda x: rnnt_amd.beam_select(x, torch.zeros(2, 3), 2), lambda x: rnnt_amd.beam_reorder(parent, [x])[0])
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_tracing_is_refused(i):
+    """A trace would record the allocation of the results alone, and return what memory happens to hold."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = _operators()[i], torch.randn(2, 3, 8)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, x, check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(x)
