@@ -82,6 +82,9 @@ Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 // Results are filled through raw pointers, past everything of torch that follows a computation; what would come out wrong without
 // a word is refused.  A dual tensor of forward-mode differentiation would lose its tangent.
+// What memory holds is what is read: a view that negates on access becomes a tensor that holds its values.
+Tensor values(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A trace would hold the allocation of the results and nothing of what is written to them.
 void refuse_tracing(const char* op) {
   TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), op,
@@ -129,8 +132,9 @@ struct Drop {
   int64_t drop16, seed, offset;  // seed and offset: the bits of unsigned values
 };
 
-Tensor run_dropout(const Tensor& given, const Drop& d, const Tensor& offset_t) {
-  Tensor x = given;
+Tensor run_dropout(const Tensor& given, const Drop& d, const Tensor& offset_given) {
+  Tensor x = values(given);
+  const Tensor offset_t = values(offset_given);
   const int64_t cols = x.size(-1);
   if (cols > kInt) bad_value("dropout: the last dimension holds 2^31 elements or more");
   int64_t stride = cols;
@@ -180,7 +184,7 @@ Tensor dropout(const Tensor& x, int64_t drop16, uint64_t seed, uint64_t offset, 
 // ---- Dense layer --------------------------------------------------------------------------------------------------------
 // t as [rows, last dimension] whose last dimension is contiguous, and the distance of its rows
 Tensor as_rows(const Tensor& given, long long* stride) {
-  Tensor t = given;
+  Tensor t = values(given);
   const int64_t n = t.size(-1);
   if (t.is_contiguous()) {
     *stride = n;
@@ -218,7 +222,7 @@ rnnt_mi355x_layer layer_of(const Tensor& x, long long x_stride, const Tensor& ke
 
 // y, and the pre-activation where it is asked for
 std::pair<Tensor, Tensor> run_layer(const Tensor& x_given, const Tensor& kernel_given, const Tensor& bias_given, const Tensor& residual_given,
-                                    const Tensor& offset_t, const LayerArgs& a, bool want_aux) {
+                                    const Tensor& offset_given, const LayerArgs& a, bool want_aux) {
   const c10::DeviceGuard guard(x_given.device());
   at::DimVector size(x_given.sizes().begin(), x_given.sizes().end());
   size.back() = kernel_given.size(1);
@@ -226,11 +230,11 @@ std::pair<Tensor, Tensor> run_layer(const Tensor& x_given, const Tensor& kernel_
   if (want_aux) aux = at::empty(size, x_given.options().dtype(x_given.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat));
   if (y.numel() == 0) return {y, aux};
   long long x_stride, kernel_stride;
-  const Tensor x = as_rows(x_given, &x_stride), kernel = as_rows(kernel_given, &kernel_stride);
+  const Tensor x = as_rows(x_given, &x_stride), kernel = as_rows(kernel_given, &kernel_stride), offset_t = values(offset_given);
   rnnt_mi355x_layer l = layer_of(x, x_stride, kernel, kernel_stride, a, offset_t);
   Tensor bias, residual;
   if (bias_given.defined()) {
-    bias = bias_given.contiguous();
+    bias = values(bias_given).contiguous();
     l.bias = bias.data_ptr();
   }
   if (residual_given.defined()) {
@@ -268,7 +272,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "dense: the gradient is not differentiable (create_graph)");
     refuse_waits_outside_capture("dense");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x_given = saved[0], &kernel_given = saved[1], &y = saved[2], &aux = saved[3], &offset_t = saved[4];
+    const Tensor &x_given = saved[0], &kernel_given = saved[1], &y = saved[2], &aux = saved[3], offset_t = values(saved[4]);
     // edges are counted over the tensors that were there
     const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2),
@@ -336,7 +340,7 @@ constexpr int64_t kMaxBeams = 64, kMaxWidth = 64;
 std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits_given, const Tensor& scores_given, int64_t width, const OptTensor& enc_,
                                                const OptTensor& allowed_, const OptTensor& finished_, int64_t end) {
   const char* op = "beam_select";
-  Tensor logits = logits_given, scores = scores_given, enc = or_none(enc_), allowed = or_none(allowed_), finished = or_none(finished_);
+  Tensor logits = values(logits_given), scores = values(scores_given), enc = values(or_none(enc_)), allowed = or_none(allowed_), finished = or_none(finished_);
   refuse_tracing(op);
   refuse_tangents(op, {&logits, &scores, &enc});
   on_gpu(op, "logits", logits);
@@ -432,7 +436,7 @@ std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<T
       if (out_given->size() != states.size()) bad_value("beam_reorder: out must be as many tensors as states");
       const Tensor& o = (*out_given)[i];
       same_device(op, ("out[" + std::to_string(i) + "]").c_str(), o, parent_given);
-      if (o.sizes() != at::IntArrayRef(size) || o.scalar_type() != s.scalar_type() || !o.is_contiguous())
+      if (o.sizes() != at::IntArrayRef(size) || o.scalar_type() != s.scalar_type() || !o.is_contiguous() || o.is_conj() || o.is_neg())
         bad_value("beam_reorder: out must be dense tensors of the results' shapes and types");
       out.push_back(o);
     }
@@ -455,7 +459,7 @@ std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<T
     for (Tensor& o : out) o.zero_();
     return out;
   }
-  const Tensor parent = parent_given.contiguous();
+  const Tensor parent = values(parent_given).contiguous();
   std::vector<rnnt_mi355x_reorder_tensor> table;
   std::vector<Tensor> keep;
   for (size_t i = 0; i < states.size(); ++i) {

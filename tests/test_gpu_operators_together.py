@@ -175,3 +175,53 @@ def test_tensors_without_memory_of_their_own_never_reach_a_kernel(i):
     with FakeTensorMode(), pytest.raises((RuntimeError, ValueError)):
         call(torch.empty(2, 3, 8, device=DEV))
     torch.cuda.synchronize()
+
+
+def _negated(t):
+    """A view whose memory holds -t."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_negated_views_give_their_values(dtype):
+    """What memory holds is not the value: dense, dropout and the beam step, each input in turn, forward and backward."""
+    g = torch.Generator().manual_seed(15)
+    def t(*s):
+        return torch.randn(s, generator=g).to(dtype).to(DEV)
+    args = {"x": t(70, 24), "kernel": t(24, 16), "bias": t(16), "residual": t(70, 16)}
+
+    def step(args, dy):
+        leaves = {n: a.detach().requires_grad_(True) for n, a in args.items()}
+        y = rnnt_amd.dense(**leaves, activation="tanh", dropout=0.2, seed=1, offset=off)
+        return (y, *torch.autograd.grad(y, list(leaves.values()), dy))
+    off, dy = torch.tensor([9], device=DEV), t(70, 16)
+    want = step(args, dy)
+    for name in args:
+        assert all(torch.equal(a, b) for a, b in zip(step({**args, name: _negated(args[name])}, dy), want)), name
+    assert all(torch.equal(a, b) for a, b in zip(step(args, _negated(dy)), want))
+    plain, off = off, _negated(off)
+    assert all(torch.equal(a, b) for a, b in zip(step(args, dy), want))
+    # one column of a complex matrix: dense as it lies, and negated
+    z = torch.randn(40, 1, dtype=torch.complex64, generator=g).to(DEV).conj().imag
+    if dtype == torch.float32:
+        assert z.is_neg()
+        k, r = t(1, 5), z.clone()
+        assert torch.equal(rnnt_amd.dense(z, k), rnnt_amd.dense(z.clone(), k))
+        assert torch.equal(rnnt_amd.dense(args["x"][:40], t(24, 1) * 0, residual=z), r)
+
+    x = args["x"].clone().requires_grad_(True)
+    y = rnnt_amd.dropout(_negated(x), 0.4, seed=3, offset=off)
+    assert torch.equal(y, rnnt_amd.dropout(x, 0.4, seed=3, offset=plain))
+    assert torch.equal(torch.autograd.grad(y, x, _negated(args["x"]))[0], rnnt_amd.dropout(args["x"], 0.4, seed=3, offset=plain))
+
+    logits, scores, enc = t(2, 3, 50), -torch.rand(2, 3, device=DEV), t(2, 50)
+    want = rnnt_amd.beam_select(logits, scores, 4, enc)
+    for i in range(3):
+        given = [_negated(a) if i == j else a for j, a in enumerate((logits, scores, enc))]
+        assert all(torch.equal(a, b) for a, b in zip(rnnt_amd.beam_select(given[0], given[1], 4, given[2]), want))
+    (moved,) = rnnt_amd.beam_reorder(want[1], [logits])
+    assert torch.equal(rnnt_amd.beam_reorder(_negated(want[1]), [_negated(logits)])[0], moved)
+    with pytest.raises(ValueError, match="out must be dense"):
+        rnnt_amd.beam_reorder(want[1], [logits], out=[torch._neg_view(torch.zeros_like(moved))])
