@@ -33,6 +33,6 @@ def beam_reorder(parent, states, batch_dim=0, out=None):
     parent: int32 [B, W] as beam_select returns it.  states: a list of tensors of any type whose dimensions batch_dim and
     batch_dim + 1 are (B, K) -- [layers, B, K, hidden] has batch_dim 1.  Returns a list with W in the place of K and row
     parent[b, w] of utterance b at [b, w]; zeros where parent is -1 (any value outside [0, K)).  out: tensors to write to
-    instead of new ones, dense, of the results' shapes and types, sharing no memory with states or one another.  Nothing is
-    differentiable here."""
+    instead of new ones, dense, of the results' shapes and types, sharing no memory with states or one another, and
+    requiring no gradients.  Nothing is differentiable here."""
     return _lib.native().beam_reorder(parent, states, batch_dim, out)

@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -452,6 +453,10 @@ std::vector<Tensor> beam_reorder(const Tensor& parent_given, const std::vector<T
         const auto a = bytes_of(out[i]), b = bytes_of(all[j]);
         if (a.first < b.second && b.first < a.second) bad_value("beam_reorder: out overlaps a state, another output or parent");
       }
+    for (const Tensor& o : out)
+      if (at::GradMode::is_enabled() && o.requires_grad()) bad_value("beam_reorder: out must not require gradients");
+    // written in place: autograd has to see it where a graph keeps one of them
+    for (const Tensor& o : out) torch::autograd::impl::bump_version(o);
   }
   if (states.empty()) return out;
   if (std::max(std::max(B, K), W) > kInt) bad_value("beam_reorder: more than 2^31 - 1 utterances or beams");

@@ -313,3 +313,27 @@ def test_beams_whose_totals_are_nearly_the_same(pieces):
     lse = torch.logsumexp(x - x.amax(2, keepdim=True), 2)[0]
     for gap in (5e-7, -5e-7):
         run(logits, torch.tensor([[(lse[0] - lse[1] + gap).item(), 0.0]]), 2, {})
+
+
+def test_reorder_into_out_is_seen_by_autograd():
+    """`out` is written in place: a graph that keeps it raises instead of using what is there now, and a tensor that requires
+    gradients is refused as any in-place write of one is."""
+    parent = torch.tensor([[2, 0], [1, 1]], dtype=torch.int32, device=DEV)
+    state, out = torch.randn(2, 3, 5, device=DEV), torch.randn(2, 2, 5, device=DEV)
+    w = torch.ones(5, device=DEV, requires_grad=True)
+    y = (out[0] * w).sum()  # a view keeps it, too
+    before = out._version
+    rnnt_amd.beam_reorder(parent, [state], out=[out])
+    assert out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    leaf = torch.zeros(2, 2, 5, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="require gradients"):
+        rnnt_amd.beam_reorder(parent, [state], out=[leaf])
+    with torch.no_grad():
+        assert torch.equal(rnnt_amd.beam_reorder(parent, [state], out=[leaf])[0], rnnt_amd.beam_reorder(parent, [state])[0])
+    with torch.inference_mode():
+        fixed = torch.zeros(2, 2, 5, device=DEV)
+        rnnt_amd.beam_reorder(parent, [state], out=[fixed])
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        rnnt_amd.beam_reorder(parent, [state], out=[fixed])
