@@ -118,12 +118,12 @@ def lib() -> ctypes.CDLL:
             try:
                 _build.hipcc_path()
             except RuntimeError:
-                raise RNNTLibraryError(f"{LIB} is older than its sources ({_build.newer_sources()}) and hipcc is not "
+                raise RNNTLibraryError(f"{LIB} is older than its sources ({_build.newer_sources()}) or built with other flags, and hipcc is not "
                                        "available to rebuild it") from None
             try:
                 _build.build()
             except (OSError, subprocess.CalledProcessError) as e:
-                raise RNNTLibraryError(f"{LIB} is older than its sources and rebuilding it failed: {e}") from e
+                raise RNNTLibraryError(f"{LIB} is older than its sources or built with other flags, and rebuilding it failed: {e}") from e
         try:
             handle = ctypes.CDLL(LIB)
         except OSError as e:
@@ -151,7 +151,7 @@ def native():
             try:
                 _build.build_native()
             except (RuntimeError, OSError, subprocess.CalledProcessError) as e:
-                raise RNNTLibraryError(f"{_build.NATIVE} is missing or older than its source and building it failed: {e}; build it with "
+                raise RNNTLibraryError(f"{_build.NATIVE} is missing, older than its source or for another torch, and building it failed: {e}; build it with "
                                        "`python -m rnnt_amd.build`") from e
         try:
             from . import _native as module

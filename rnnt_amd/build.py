@@ -27,6 +27,8 @@ NATIVE = os.path.join(_HERE, "_native.so")
 # hipcc's packed float32 instructions have given wrong results on this hardware now and then: no source is built with them
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Xclang", "-target-feature", "-Xclang",
          "-packed-fp32-ops"]
+# the HIP headers and torch's want to be told their platform
+NATIVE_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
 
 
 def sources_digest() -> str:
@@ -47,11 +49,34 @@ def hipcc_path() -> str:
     raise RuntimeError("hipcc not found: cannot build librnnt_mi355x.so")
 
 
+def _stamp(*what) -> str:
+    """What an artefact depends on besides its sources, as the bytes that it carries."""
+    import hashlib
+    return "rnnt-build-" + hashlib.sha256("\0".join(what).encode()).hexdigest()[:16]
+
+
+def lib_stamp() -> str:
+    return _stamp(*FLAGS)
+
+
+def native_stamp() -> str:
+    """The binding is built against one torch and one Python."""
+    import sysconfig
+
+    import torch
+    return _stamp(torch.__version__, str(torch.version.git_version), str(sysconfig.get_config_var("SOABI")), *NATIVE_FLAGS)
+
+
+def _carries(path: str, stamp: str) -> bool:
+    with open(path, "rb") as f:
+        return stamp.encode() in f.read()
+
+
 def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(p) > t for p in (*SOURCES, *PIECES, *OPERATOR_SOURCES, *OPERATOR_PIECES, HEADER))
+    return not _carries(LIB, lib_stamp()) or any(os.path.getmtime(p) > t for p in (*SOURCES, *PIECES, *OPERATOR_SOURCES, *OPERATOR_PIECES, HEADER))
 
 
 def newer_sources():
@@ -66,7 +91,7 @@ def needs_native_build() -> bool:
     if not os.path.exists(NATIVE):
         return True
     t = os.path.getmtime(NATIVE)
-    return any(os.path.getmtime(p) > t for p in (BINDING, HEADER))
+    return not _carries(NATIVE, native_stamp()) or any(os.path.getmtime(p) > t for p in (BINDING, HEADER))
 
 
 def native_command(out: str):
@@ -83,8 +108,7 @@ def native_command(out: str):
         raise RuntimeError("g++ not found: cannot build the torch binding")
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"),
                sysconfig.get_path("include")]
-    # the HIP headers and torch's want to be told their platform
-    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    return [cxx, *NATIVE_FLAGS, f'-DRNNT_BUILD_STAMP="{native_stamp()}"',
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include], BINDING, "-o", out,
             f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
 
@@ -128,7 +152,7 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB
         try:
             if not force and out == LIB and not needs_build():  # another process built it while this one waited
                 return LIB
-            flags = [*FLAGS, *[f"-D{d}" for d in defines]]
+            flags = [*FLAGS, f'-DRNNT_BUILD_STAMP="{lib_stamp()}"', *[f"-D{d}" for d in defines]]
             with tempfile.TemporaryDirectory(prefix=".build-", dir=os.path.dirname(out)) as tmp:
                 # one object per source, compiled side by side, then one link
                 sources = [*SOURCES, *OPERATOR_SOURCES]

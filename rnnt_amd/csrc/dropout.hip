@@ -5,6 +5,10 @@
 
 namespace {
 
+#ifdef RNNT_BUILD_STAMP
+__attribute__((used)) const char kBuildStamp[] = RNNT_BUILD_STAMP;  // the flags all sources were compiled with: build.py looks for it
+#endif
+
 constexpr int kThreads = 256;
 constexpr int kGroups = 4;  // groups of eight elements per thread, all loaded before the first draw
 

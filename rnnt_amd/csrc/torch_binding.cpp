@@ -24,6 +24,10 @@ using OptTensor = std::optional<Tensor>;
 
 namespace {
 
+#ifdef RNNT_BUILD_STAMP
+__attribute__((used)) const char kBuildStamp[] = RNNT_BUILD_STAMP;  // the torch and Python this is for: build.py looks for it
+#endif
+
 struct Entries {
   decltype(&rnnt_mi355x_dropout) dropout;
   decltype(&rnnt_mi355x_layer_workspace_bytes) layer_workspace_bytes;

@@ -212,3 +212,23 @@ def test_tracing_is_refused(i):
         torch.jit.trace(call, x, check_trace=False)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(call)(x)
+
+
+def test_artefacts_built_another_way_are_stale(monkeypatch):
+    """Besides their sources' times: the library's flags, and the torch and Python that the binding was compiled for."""
+    import sysconfig
+
+    from rnnt_amd import build
+    _lib.native()  # builds what is missing
+    assert not build.needs_build() and not build.needs_native_build()
+    with monkeypatch.context() as m:
+        m.setattr(build, "FLAGS", [*build.FLAGS, "-DANOTHER"])
+        assert build.needs_build() and not build.needs_native_build()
+    for target, name, value in ((torch, "__version__", "9.9"), (torch.version, "git_version", "0" * 40)):
+        with monkeypatch.context() as m:
+            m.setattr(target, name, value)
+            assert build.needs_native_build() and not build.needs_build()
+    with monkeypatch.context() as m:
+        m.setattr(sysconfig, "get_config_var", lambda name: "another")
+        assert build.needs_native_build()
+    assert not build.needs_build() and not build.needs_native_build()
