@@ -365,3 +365,11 @@ def test_gelu_keeps_its_digits_in_the_negative_tail(dtype, rows):
     rel = (5.25 * f * f + 24) * 3 * 2.0 ** -24 + (0 if dtype == torch.float32 else U[dtype] * 2.02)
     far = f <= -1.2
     assert (np.abs(f64(dx)[:, 0] - slope) <= rel * np.abs(slope) + 2 * LEAST[dtype])[far].all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,N,act,rate", [(3500, 3400, 136, "silu", 0.1), (9000, 2000, 2100, "gelu", 0.0), (3333, 3531, 205, "linear", 0.0)])
+def test_gradients_in_the_largest_blocks(M, K, N, act, rate, dtype):
+    """Blocks of 256 x 256 begin at 192 of them: for dx 14 x 14 over rows and inputs (3500 x 3400; 3333 x 3531 with every operand
+    packed), for the kernel 8 x 9 over inputs and outputs (2000 x 2100) times 3 pieces of 4096 of the 9000 rows, tiles cut along them and joined."""
+    check_layer(M, K, N, dtype, act, True, False, rate)
