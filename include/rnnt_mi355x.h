@@ -267,7 +267,8 @@ int rnnt_mi355x_dropout(const void* x, long long x_stride, void* y, long long ro
  * (d residual is dy).  x: [rows, in], kernel: [in, out] (Keras), residual, y, aux,
  * dy: [rows, out]; all of one `dtype`, last dimension contiguous, rows *_stride elements
  * apart (y and aux dense).  float32 products are accurate to float32 rounding (three
- * bfloat16 parts an operand), sums are float32.  bias, residual and aux may be NULL.
+ * bfloat16 parts an operand; operands below 2^-102 lose their last places), sums are
+ * float32; in 16 bits dz is rounded to the type before its two products.  bias, residual and aux may be NULL.
  * act: RNNT_MI355X_ACT_*; gelu is z Phi(z), off by (24 + 2 z^2) 2^-24 of itself in float32 and by 2^-13 (2^-9.8 below
  * z = -5.9) next to the type's rounding in 16 bits; results below 2^-122 may be 0.  Dropout as rnnt_mi355x_dropout
  * draws it for [rows, out] (drop16 0: none).

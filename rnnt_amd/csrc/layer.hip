@@ -88,7 +88,10 @@ __global__ __launch_bounds__(256) void k_layer_pack(PackArgs a, PackArgs b) {
   else pack_block(b, blockIdx.x - a.blocks);
 }
 
-// dz, its column sums, and the copies of the operands that lie badly: what the gradient's products begin with.  Bound by
+// dz, its column sums, and the copies of the operands that lie badly: what the gradient's products begin with.  In 16-bit layers
+// dz is rounded to the type, as the matrix instruction takes it: a rounding next to the result's own, so that the gradients'
+// relative error (2-norm, against float64) is 2.9e-4 instead of 2.1e-4 in float16 and 2.3e-3 instead of 1.7e-3 in bfloat16.  dz in two parts
+// would keep it and double both products.  The column sums take it unrounded.  Bound by
 // memory, dy and the saved tensor read once and dz written once (49200 x 250 float32, tanh and dropout: 28 us = 5.3 TB/s), or by
 // the slope and the generator where elements are small (32768 x 4096 bfloat16, gelu and dropout: 185 us = 4.3 TB/s).
 template <class T>
@@ -354,9 +357,10 @@ Plan plan_product(int product, int dtype, int M, int N, int K, bool direct) {
     p.bn = 64;
     p.tiles_m = 1;
     if (product == kForward && direct && M > 32 && K <= 2048 && ceil_div(N, 32) <= kCUs) {
-      // Columns halved instead of k cut, while every block reading all of x costs less than a join.  Thin against wide, 64 rows in
-      // bfloat16: 2048 x 8192 14.9 us (16.2), 512 x 4096 6.6 (7.3), 256 x 8192 6.0 (6.7); 4096 x 4096 18.4 (16.3), 8192 x 2048 19.0 (17.4);
-      // 16 rows 1024 x 4096 7.9 (7.7).
+      // Columns halved instead of k cut, while every block reading all of x costs less than a join.  Thin against wide, us a call:
+      // 64 rows in bfloat16, weights that come from memory: 2048 x 8192 17.2 (17.2), 2560 x 8192 21.2 (19.7), 3584 x 8192 26.1 (23.0);
+      // 2560 x 4096 16.6 (18.4), 3584 x 4096 19.3 (18.4), 4096 x 4096 21.4 (17.6); 48 rows in float16 1024 x 8192 10.1 (11.5).  Weights that
+      // the caches hold: 2048 x 8192 12.6 (14.1), 512 x 4096 6.6 (7.3), 256 x 8192 6.0 (6.7).  16 rows 1024 x 4096 7.9 (7.7).
       p.block = kBlock64Thin;
       p.bn = 32;
     }

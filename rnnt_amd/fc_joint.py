@@ -16,8 +16,9 @@ additive one and goes straight to the fused additive-joint loss, so not even
 [B,T,U+1,V] is formed.  The following layers multiply a [B*T*(U+1), hidden]
 matrix by a small kernel: up to 128 x 128 they run on hand-written tall-skinny
 MFMA kernels (weights resident in LDS), beyond that on the library GEMM.  With dropout (training-time noise,
-keras_model.py:102-103) the hidden layers run as ``dense``, which draws the mask
-in its epilogue and again in its backward pass, at any width.
+keras_model.py:102-103) the layers between the first and the last run as ``dense``,
+in float32, which draws the mask in its epilogue and again in its backward pass, at
+any width.
 """
 from __future__ import annotations
 
@@ -116,7 +117,7 @@ def joint_dense(x, kernel, bias, activation="linear"):
     """One TimeDistributed(Dense) of get_fc (keras_model.py:88-101) over x[..., K]:
     activation(x @ kernel[K,N] + bias[N]), "linear" or "tanh".  Widths up to
     DENSE_MAX_DIM run on the hand-written tall-skinny kernels; wider layers go
-    to the library GEMM, which is efficient there."""
+    to the library GEMM (``dense`` is the hand-written layer at any width)."""
     if activation not in ("linear", "tanh"):
         raise ValueError("joint_dense: activation must be 'linear' or 'tanh'")
     K, N = kernel.shape

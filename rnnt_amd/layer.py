@@ -16,10 +16,11 @@ def dense(x, kernel, bias=None, activation="linear", residual=None, dropout=0.0,
     """residual + dropout(activation(x @ kernel + bias)), differentiable in x, kernel, bias and residual.
 
     x [..., in], kernel [in, out] (Keras layout), bias [out], residual [..., out]: one of float32, bfloat16, float16, the same
-    for all; the result has that type, products and sums are float32 throughout (float32 inputs included).  activation:
-    "linear", "tanh", "relu", "gelu" (z times the normal distribution's function, its error relative to the
-    result also in the negative tail) or "silu".  dropout, seed, offset: as
-    ``rnnt_amd.dropout`` takes them, the mask being the one it draws for the result; rate 0 at inference.
+    for all; the result has that type.  Products of float32 inputs are float32's, and sums are float32 throughout.  activation:
+    "linear", "tanh", "relu", "gelu" (z times the normal distribution's function) or "silu", with errors relative to the
+    result, below 2^-17 of it in float32 up to |z| = 5.  In 16 bits the gradient of the pre-activation is rounded to the type before its
+    two products, as the result is before it leaves.  dropout, seed, offset: as ``rnnt_amd.dropout`` takes them, the mask being the
+    one it draws for the result; rate 0 at inference.
 
     The same inputs give the same bits, forward and backward.  The gradient is not differentiable itself (create_graph is
     refused), and forward-mode differentiation is refused."""
