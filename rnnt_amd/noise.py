@@ -16,7 +16,7 @@ from ._operator import drop16, seed_offset
 def dropout(x, rate, seed=0, offset=0):
     """x with elements dropped at `rate` (rounded to steps of 2^-16) and the others scaled by 1 / (1 - rate).
 
-    x: float32, bfloat16 or float16, any shape.  seed: an integer below 2^64.  offset: an integer below 2^64, or one int64
+    x: float32, bfloat16 or float16, any shape whose last dimension is below 2^31.  seed: an integer below 2^64.  offset: an integer below 2^64, or one int64
     on the device (read by the kernel: inside a captured graph the caller advances it between replays); calls that need
     independent masks take different offsets.  rate 0 returns x itself.  Differentiable any number of times, backward; forward-mode
     differentiation is refused."""
